@@ -6,8 +6,25 @@
 #include <map>
 
 #include "agb.h"
+#include "bindings.h"
+
+namespace agb_python {
+
+torch::Tensor status_word(int device) {
+  static std::map<int, torch::Tensor> words;
+  auto it = words.find(device);
+  if (it == words.end()) {
+    auto w = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, device));
+    it = words.emplace(device, w).first;
+  }
+  return it->second;
+}
+
+}  // namespace agb_python
 
 namespace {
+
+using agb_python::status_word;
 
 using torch::Tensor;
 
@@ -17,18 +34,6 @@ cudaStream_t stream_of(const Tensor& t) {
 
 void check(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e), " (", agb::error_detail(), ")");
-}
-
-// One int32 status word per device; kernels write a non-zero code when a bounded wait
-// ran out or an argument was rejected on the device.
-Tensor status_word(int device) {
-  static std::map<int, Tensor> words;
-  auto it = words.find(device);
-  if (it == words.end()) {
-    auto w = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, device));
-    it = words.emplace(device, w).first;
-  }
-  return it->second;
 }
 
 int sm_count(int device) { return at::cuda::getDeviceProperties(device)->multiProcessorCount; }
@@ -1129,4 +1134,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tp_signal_done", &tp_signal_done);
   m.def("exchange", &exchange);
   m.def("status", &status);
+  agb_python::bind_packed(m);
 }

@@ -55,8 +55,8 @@ constexpr size_t kMaxCachedMaps = 1 << 14;
 void set_error_detail(const char* text) { g_detail = text; }
 const char* error_detail() { return g_detail; }
 
-bool make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                          const uint64_t* strides_bytes, const uint32_t* box) {
+bool encode_tensor_map_16bit(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                             const uint64_t* strides_bytes, const uint32_t* box) {
   EncodeFn fn = encode_fn();
   if (!fn) return false;
   // The driver call needs a current context; a thread that has only used the runtime API
@@ -67,20 +67,6 @@ bool make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const ui
     bound = true;
   }
   if (rank < 1 || rank > 5) return false;
-  MapKey key{};
-  key.words[0] = reinterpret_cast<uint64_t>(base);
-  key.words[1] = uint64_t(rank);
-  for (int i = 0; i < rank; ++i) {
-    key.words[2 + i] = dims[i];
-    key.words[11 + i] = box[i];
-  }
-  for (int i = 0; i + 1 < rank; ++i) key.words[7 + i] = strides_bytes[i];
-  static thread_local std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  auto found = cache.find(key);
-  if (found != cache.end()) {
-    *map = found->second;
-    return true;
-  }
   cuuint64_t gdims[5];
   cuuint64_t gstrides[4];
   cuuint32_t gbox[5];
@@ -104,6 +90,27 @@ bool make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const ui
     set_error_detail(text);
     return false;
   }
+  return true;
+}
+
+bool make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box) {
+  if (rank < 1 || rank > 5) return false;
+  MapKey key{};
+  key.words[0] = reinterpret_cast<uint64_t>(base);
+  key.words[1] = uint64_t(rank);
+  for (int i = 0; i < rank; ++i) {
+    key.words[2 + i] = dims[i];
+    key.words[11 + i] = box[i];
+  }
+  for (int i = 0; i + 1 < rank; ++i) key.words[7 + i] = strides_bytes[i];
+  static thread_local std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
+  auto found = cache.find(key);
+  if (found != cache.end()) {
+    *map = found->second;
+    return true;
+  }
+  if (!encode_tensor_map_16bit(map, base, rank, dims, strides_bytes, box)) return false;
   if (cache.size() >= kMaxCachedMaps) cache.clear();
   cache.emplace(key, *map);
   return true;

@@ -15,4 +15,9 @@ namespace agb {
 bool make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                           const uint64_t* strides_bytes, const uint32_t* box);
 
+// The same for bf16 or fp16, encoded anew for every call (a box may be less than one swizzle span
+// wide only in dims[0], where the rest of the span reads as zero).
+bool encode_tensor_map_16bit(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                             const uint64_t* strides_bytes, const uint32_t* box);
+
 }  // namespace agb

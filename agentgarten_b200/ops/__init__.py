@@ -18,6 +18,7 @@ import torch.autograd.forward_ad as fwAD
 from . import native, reference
 from .attention import attention, attention_jvp, planned_attention
 from .linear import adjoin, joined, joint_linear, linear, linear_residual, rows_linear
+from .packed import RotaryFrequencies, packed_attention, rotary_embed, rotary_frequencies
 from .pointwise import (
     gated_residual,
     head_norm_rope,
@@ -33,6 +34,7 @@ from .pointwise import (
 )
 
 __all__ = [
+    "RotaryFrequencies",
     "adjoin",
     "attention",
     "attention_jvp",
@@ -44,6 +46,7 @@ __all__ = [
     "linear_residual",
     "native",
     "norm_modulate",
+    "packed_attention",
     "planned_attention",
     "reference",
     "rf_interpolate",
@@ -53,6 +56,8 @@ __all__ = [
     "rows_linear",
     "rms_norm_add",
     "rotary",
+    "rotary_embed",
+    "rotary_frequencies",
     "silu_mul",
     "silu_mul_pair",
 ]

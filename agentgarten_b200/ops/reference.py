@@ -24,6 +24,7 @@ __all__ = [
     "attention_jvp",
     "head_norm_rope",
     "linear",
+    "packed_attention",
     "relocate_rows",
     "rf_interpolate",
     "rf_x0",
@@ -31,6 +32,7 @@ __all__ = [
     "rms_norm_add",
     "rotate_half",
     "rotary",
+    "rotary_embed",
     "silu_mul",
 ]
 
@@ -69,6 +71,26 @@ def head_norm_rope(value: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor,
     return rotary(rms_norm(value, weight, eps), cos, sin)
 
 
+def rotary_embed(value: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, amplitude: float = 1.0,
+                 axis: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor:
+    """``value`` ``[..., heads, dim]`` turned by ``2 pi * positions * turns`` (angles in FP64, the turn in
+    at least FP32, one rounding); elements behind ``2 * len(turns)`` are copied."""
+    where = positions.double()[..., None] if axis is None else positions.double()[..., axis.long()]
+    angle = where * turns
+    angle = (angle - angle.round()) * (2 * math.pi)
+    wide = torch.promote_types(value.dtype, torch.float32)
+    cos, sin = ((f(angle) * amplitude).to(wide).unsqueeze(-2) for f in (torch.cos, torch.sin))
+    slots = turns.shape[0]
+    head = value[..., : 2 * slots].to(wide)
+    if interleaved:
+        a, b = head[..., 0::2], head[..., 1::2]
+        head = torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2)
+    else:
+        a, b = head[..., :slots], head[..., slots:]
+        head = torch.cat((a * cos - b * sin, a * sin + b * cos), dim=-1)
+    return torch.cat((head.to(value.dtype), value[..., 2 * slots:]), dim=-1)
+
+
 def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return F.silu(gate) * up
 
@@ -101,6 +123,39 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
         attn_mask=mask, is_causal=causal, enable_gqa=q.shape[2] != k.shape[2])
     return out.transpose(1, 2)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
+                     k_offsets: torch.Tensor, k_lengths: torch.Tensor | None, scale: float) -> torch.Tensor:
+    """Causal attention of packed ``[total, heads, dim]`` sequences whose queries are the last rows of
+    their keys, in at least FP32 with one rounding; rows without a visible key and rows behind the last
+    sequence are zero."""
+    wide = torch.promote_types(q.dtype, torch.float32)
+    group = q.shape[1] // k.shape[1]
+    starts, key_starts = q_offsets.tolist(), k_offsets.tolist()
+    lengths = [b - a for a, b in zip(key_starts, key_starts[1:])] if k_lengths is None else k_lengths.tolist()
+    if starts[0] or key_starts[0] or starts[-1] > q.shape[0] or key_starts[-1] > k.shape[0] or any(
+            b < a or not 0 <= n <= d - c for a, b, c, d, n in
+            zip(starts, starts[1:], key_starts, key_starts[1:], lengths)):
+        raise ValueError("packed_attention: offsets start at 0, never fall and lie inside the tensors")
+    pieces = []
+    for q0, q1, k0, keys in zip(starts, starts[1:], key_starts, lengths):
+        rows = q1 - q0
+        if rows == 0:
+            continue
+        qs = q[q0:q1].to(wide).transpose(0, 1)
+        ks, vs = (t[k0:k0 + keys].to(wide).transpose(0, 1).repeat_interleave(group, 0) for t in (k, v))
+        s = qs @ ks.transpose(-1, -2) * scale
+        seen = torch.arange(keys, device=q.device)[None] <= torch.arange(rows, device=q.device)[:, None] + (keys - rows)
+        # subtracting a constant keeps the quotient; rows without a key divide 0 by 1
+        s = s.masked_fill(~seen, float("-inf"))
+        top = s.detach().amax(-1, keepdim=True) if keys else s.new_zeros(*s.shape[:-1], 1)
+        p = torch.exp(s - top.masked_fill(top == float("-inf"), 0.0))
+        total = p.sum(-1, keepdim=True)
+        p = p / torch.where(seen.any(-1)[:, None], total, torch.ones_like(total))
+        pieces.append((p @ vs).transpose(0, 1).to(q.dtype))
+    pieces.append(q.new_zeros(q.shape[0] - starts[-1], *q.shape[1:]))
+    return torch.cat(pieces)
 
 
 def attention_jvp(q, k, v, dq, dk, dv, key_mask=None):

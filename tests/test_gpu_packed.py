@@ -1,0 +1,245 @@
+"""Rotary positions and packed causal attention on the kernels, against 64-bit definitions."""
+
+import math
+
+import pytest
+import torch
+
+from agentgarten_b200 import ops
+from agentgarten_b200.ops import native
+
+import packed_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _status():
+    torch.cuda.synchronize()
+    return int(native.ext().status(torch.cuda.current_device()).item())
+
+
+# --------------------------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("dtype", [BF16, FP16, torch.float32])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,turned", [
+    (1, 32, 8, 128, 128), (3, 4, 2, 64, 32), (37, 3, 1, 80, 20), (130, 5, 5, 96, 96), (9, 2, 2, 6, 2),
+    (1000, 32, 8, 128, 64), (5, 1, 1, 256, 128), (2, 3, 1, 7, 4)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary(dtype, tokens, heads, kv_heads, dim, turned, interleaved):
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    q, k = (torch.randn(tokens, h, dim, device=DEV, generator=g).to(dtype) for h in (heads, kv_heads))
+    positions = torch.randint(0, 1 << 20, (tokens,), device=DEV, generator=g)
+    f = ops.rotary_frequencies(turned, 5e6, scaling="yarn", factor=8.0, trained_positions=4096, device=DEV)
+    before = native.launches()
+    got = ops.rotary_embed(q, k, positions, f, interleaved=interleaved)
+    assert native.launches() == before + 1
+    for out, x in zip(got, (q, k)):
+        oracle.assert_close(out, *oracle.rotary(x, positions, f.turns * 2 * math.pi, f.amplitude, interleaved=interleaved))
+        assert torch.equal(out[..., turned:], x[..., turned:])
+
+
+def test_rotary_positions_of_every_type_and_axes():
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q = torch.randn(2, 50, 4, 128, device=DEV, generator=g).bfloat16()
+    k = torch.randn(2, 50, 2, 128, device=DEV, generator=g).bfloat16()
+    inverse = ops.rotary_frequencies(128, 5e6, device=DEV).turns * 2 * math.pi
+    whole = torch.randint(0, 1 << 30, (2, 50), device=DEV, generator=g)
+    f = ops.rotary_frequencies(128, 5e6, device=DEV)
+    for positions in (whole, whole.int(), -whole, whole + (1 << 40), whole.float() / 3):
+        for out, x in zip(ops.rotary_embed(q, k, positions, f), (q, k)):
+            # 2^40 positions are 2^38 turns: the fraction is exact to 2^-15 of a turn in 64 bits
+            extra = 2 * math.pi * 2.0 ** -15 * 2 if int(positions.abs().max()) > 1 << 31 else 0.0
+            value, bound = oracle.rotary(x, positions, inverse)
+            oracle.assert_close(out, value, bound + extra * x.double().abs().amax())
+    f = ops.rotary_frequencies(128, 5e6, sections=(24, 20, 20), device=DEV)
+    positions = torch.rand(2, 50, 3, device=DEV, generator=g) * 20000
+    for out, x in zip(ops.rotary_embed(q, k, positions, f), (q, k)):
+        oracle.assert_close(out, *oracle.rotary(x, positions, inverse, axis=f.axis))
+
+
+def test_rotary_strides():
+    """Column slices of a joint projection, transposed heads, odd alignments: read in place or copied."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    joint = torch.randn(33, 6 * 64 + 4, device=DEV, generator=g).bfloat16()
+    positions = torch.arange(33, device=DEV)
+    f = ops.rotary_frequencies(64, 1e4, device=DEV)
+    inverse = f.turns * 2 * math.pi
+    for shift in (0, 1, 2, 4):
+        q = joint[:, shift:shift + 256].unflatten(-1, (4, 64))
+        k = joint[:, 256:384].unflatten(-1, (2, 64)).transpose(0, 1).contiguous().transpose(0, 1)
+        for out, x in zip(ops.rotary_embed(q, k, positions, f), (q, k)):
+            assert out.is_contiguous()
+            oracle.assert_close(out, *oracle.rotary(x, positions, inverse))
+    x = torch.randn(33, 1, 64, device=DEV, generator=g).expand(33, 3, 64)
+    oracle.assert_close(ops.rotary_embed(x, None, positions, f)[0], *oracle.rotary(x, positions, inverse))
+    x = torch.randn(4, 6, 2, 64, device=DEV, generator=g)[::2, ::3]
+    at = torch.arange(4, device=DEV).view(2, 2)
+    oracle.assert_close(ops.rotary_embed(x, None, at, f)[0], *oracle.rotary(x, at, inverse))
+    empty = torch.randn(0, 4, 64, device=DEV)
+    assert ops.rotary_embed(empty, empty, positions[:0], f)[1].shape == empty.shape
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_gradients(dtype, interleaved):
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q, k, gq, gk = (torch.randn(21, h, 64, device=DEV, generator=g).to(dtype) for h in (4, 2, 4, 2))
+    f = ops.rotary_frequencies(32, 1e4, scaling="yarn", factor=4.0, trained_positions=64, device=DEV)
+    inverse, at = f.turns * 2 * math.pi, torch.arange(21, device=DEV)
+    q.requires_grad_()
+    k.requires_grad_()
+    out = ops.rotary_embed(q, k, at, f, interleaved=interleaved)
+    for got, x in zip(torch.autograd.grad(out, (q, k), (gq, gk), retain_graph=True), (gq, gk)):
+        oracle.assert_close(got, *oracle.rotary(x, at, -inverse, f.amplitude, interleaved=interleaved))
+    # only one output used, and a broadcast gradient
+    (got,) = torch.autograd.grad(out[1].sum(), (k,))
+    oracle.assert_close(got, *oracle.rotary(torch.ones_like(k), at, -inverse, f.amplitude, interleaved=interleaved))
+
+
+def test_rotary_device_and_type_refusals():
+    q = torch.randn(4, 2, 64, device=DEV)
+    f = ops.rotary_frequencies(64, device=DEV)
+    with pytest.raises(ValueError, match="one device"):
+        ops.rotary_embed(q, None, torch.arange(4), f)
+    with pytest.raises(ValueError, match="one device"):
+        ops.rotary_embed(q, None, torch.arange(4, device=DEV), ops.rotary_frequencies(64))
+    with pytest.raises(TypeError):
+        ops.rotary_embed(q.to(torch.float8_e4m3fn), None, torch.arange(4, device=DEV), f)
+
+
+# ------------------------------------------------------------------------------------ attention
+def _offsets(lengths):
+    at = [0]
+    for n in lengths:
+        at.append(at[-1] + n)
+    return torch.tensor(at, dtype=torch.int32, device=DEV)
+
+
+def _case(q_lengths, k_lengths, heads, kv_heads, dim, dtype, room=0, behind=0, seed=0, stale=float("nan")):
+    """Packed tensors; key rows that are no keys (room behind a sequence, rows behind the last) hold ``stale``."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rooms = [n + room for n in k_lengths]
+    q = torch.randn(sum(q_lengths) + behind, heads, dim, device=DEV, generator=g).to(dtype)
+    k, v = (torch.randn(sum(rooms) + behind, kv_heads, dim, device=DEV, generator=g).to(dtype) for _ in range(2))
+    qo, ko = _offsets(q_lengths), _offsets(rooms)
+    spans = list(zip(qo.tolist(), q_lengths, ko.tolist(), k_lengths))
+    used = torch.zeros(k.shape[0], dtype=torch.bool, device=DEV)
+    for _, _, k0, n in spans:
+        used[k0:k0 + n] = True
+    k[~used], v[~used] = stale, stale
+    q[sum(q_lengths):] = stale
+    return q, k, v, qo, ko, torch.tensor(k_lengths, dtype=torch.int32, device=DEV), spans
+
+
+def _check_forward(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw):
+    q, k, v, qo, ko, kl, spans = _case(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw)
+    before = native.launches()
+    out = ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    assert native.launches() > before
+    assert _status() == 0
+    oracle.assert_close(out, *oracle.attention(q, k, v, spans, dim ** -0.5)["out"])
+    assert not out[sum(q_lengths):].any()
+    return q, k, v, qo, ko, kl, out
+
+
+PROMPTS = [[1], [2, 1], [17], [127, 128, 129], [300, 0, 5, 514], [0], [256, 257, 1, 640]]
+
+
+@pytest.mark.parametrize("lengths", PROMPTS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (6, 2), (8, 1)])
+def test_attention_of_prompts(lengths, heads, kv_heads):
+    _check_forward(lengths, lengths, heads, kv_heads, 128, BF16, behind=7)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [8, 40, 64, 72, 80, 96, 120, 128])
+def test_attention_head_sizes_and_types(dim, dtype):
+    _check_forward([130, 3, 200], [130, 3, 200], 4, 2, dim, dtype, behind=1)
+
+
+@pytest.mark.parametrize("q_lengths,k_lengths", [
+    ([5, 100], [700, 333]), ([300], [301]), ([129, 1, 64], [129, 900, 70]), ([200], [1111]),
+    ([50, 140, 10], [20, 100, 0]),        # more queries than keys: the first rows see nothing
+    ([64, 3], [0, 0])])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (5, 5)])
+def test_attention_of_continued_prompts(q_lengths, k_lengths, heads, kv_heads):
+    _check_forward(q_lengths, k_lengths, heads, kv_heads, 128, BF16, room=13, behind=300)
+
+
+@pytest.mark.parametrize("k_lengths", [[1], [15, 16, 17, 31], [100, 0, 1, 2049], [5000], [257] * 40])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 4, 64), (32, 1, 96), (40, 2, 80)])
+def test_attention_of_single_tokens(k_lengths, heads, kv_heads, dim):
+    _check_forward([1] * len(k_lengths), k_lengths, heads, kv_heads, dim, BF16, room=21, behind=2)
+
+
+def test_attention_of_few_tokens_and_idle_sequences():
+    _check_forward([0, 1, 3, 0, 2], [40, 900, 33, 7, 2], 8, 2, 128, FP16, room=5, behind=1)
+    _check_forward([1] * 30 + [40], [200] * 30 + [300], 8, 2, 128, BF16)
+
+
+def test_attention_of_nothing():
+    q = torch.randn(6, 4, 64, device=DEV).bfloat16()
+    k = torch.randn(0, 2, 64, device=DEV).bfloat16()
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert not ops.packed_attention(q, k, k, none, none).any()
+    assert not ops.packed_attention(q, k, k, torch.tensor([0, 6], dtype=torch.int32, device=DEV),
+                                    torch.tensor([0, 0], dtype=torch.int32, device=DEV)).any()
+    k = torch.randn(9, 2, 64, device=DEV).bfloat16()
+    assert not ops.packed_attention(q, k, k, none, none).any()
+    assert ops.packed_attention(q[:0], k, k, none, none).shape == (0, 4, 64)
+    assert _status() == 0
+
+
+def test_attention_strides():
+    """Slices of a joint projection and head-major storage are read in place; others are copied."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    lengths = [70, 200]
+    joint = torch.randn(270, (8 + 2 + 2) * 64 + 8, device=DEV, generator=g).bfloat16()
+    spans = [(0, 70, 0, 70), (70, 200, 70, 200)]
+    for shift in (0, 8, 3):
+        q, k, v = (joint[:, shift + a:shift + b].unflatten(-1, (-1, 64)) for a, b in ((0, 512), (512, 640), (640, 768)))
+        out = ops.packed_attention(q, k, v, _offsets(lengths))
+        oracle.assert_close(out, *oracle.attention(q, k, v, spans, 0.125)["out"])
+    q, k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v))
+    out = ops.packed_attention(q, k, v, _offsets(lengths))
+    oracle.assert_close(out, *oracle.attention(q, k, v, spans, 0.125)["out"])
+    k = k[:, :1].expand(270, 2, 64)
+    out = ops.packed_attention(q, k, v, _offsets(lengths))
+    oracle.assert_close(out, *oracle.attention(q, k, v, spans, 0.125)["out"])
+    assert _status() == 0
+
+
+def test_attention_scores_far_from_zero():
+    """Large scores with a maximum that keeps growing along the keys: the running rescale."""
+    q, k, v, qo, ko, kl, spans = _case([300, 1], [700, 700], 4, 2, 128, BF16)
+    k *= torch.linspace(0.1, 12, k.shape[0], device=DEV)[:, None, None].to(BF16)
+    q *= 4
+    out = ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    # scores up to some hundreds, each an FP32 sum: 2^-24 * |s| * log2(e) in the exponent
+    value, bound = oracle.attention(q, k, v, spans, 128 ** -0.5)["out"]
+    oracle.assert_close(out, value, bound + 2.0 ** -24 * 2048 * v.double().abs().amax())
+    assert _status() == 0
+
+
+def test_attention_results_do_not_depend_on_company():
+    """A sequence gives bit for bit the same alone and among others (and on every run)."""
+    q, k, v, qo, ko, kl, spans = _case([130, 300, 77], [130, 300, 77], 4, 2, 128, BF16)
+    out = ops.packed_attention(q, k, v, qo)
+    assert torch.equal(out, ops.packed_attention(q, k, v, qo))
+    for q0, n, _, _ in spans:
+        alone = ops.packed_attention(q[q0:q0 + n], k[q0:q0 + n], v[q0:q0 + n], _offsets([n]))
+        assert torch.equal(alone, out[q0:q0 + n])
+
+
+@pytest.mark.parametrize("rows", [1, 140])
+def test_attention_reports_bad_offsets(rows):
+    """Offsets that leave the tensors are caught by the kernels' own checks: the sequence is skipped."""
+    q, k, v, qo, ko, kl, spans = _case([rows, rows], [200, 200], 4, 2, 64, BF16)
+    for bad in (dict(q_offsets=_offsets([rows, rows + 5])), dict(k_offsets=_offsets([200, 250])),
+                dict(k_lengths=kl + 1), dict(k_lengths=-kl), dict(q_offsets=_offsets([rows, -1]))):
+        given = dict(q_offsets=qo, k_offsets=ko, k_lengths=kl)
+        given.update(bad)
+        ops.packed_attention(q, k, v, given["q_offsets"], given["k_offsets"], k_lengths=given["k_lengths"])
+        assert _status() == 7, bad
+        native.ext().status(torch.cuda.current_device()).zero_()
