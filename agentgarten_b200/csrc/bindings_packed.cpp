@@ -127,11 +127,40 @@ std::tuple<Tensor, Tensor> packed_attention_fwd(const Tensor& query, const Tenso
   return {out, lse};
 }
 
+std::tuple<Tensor, Tensor, Tensor> packed_attention_bwd(
+    const Tensor& grad_out, const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& out,
+    const Tensor& lse, const Tensor& q_offsets, const Tensor& k_offsets, const c10::optional<Tensor>& k_lengths,
+    double scale) {
+  c10::cuda::CUDAGuard guard(query.device());
+  Tensor dq = torch::empty(query.sizes(), query.options());
+  Tensor dk = torch::empty(key.sizes(), key.options());
+  Tensor dv = torch::empty(value.sizes(), value.options());
+  if (query.numel() == 0 || key.size(0) == 0 || q_offsets.size(0) == 1) {
+    dq.zero_();
+    dk.zero_();
+    dv.zero_();
+    return {dq, dk, dv};
+  }
+  const Tensor q = mappable(query), k = mappable(key), v = mappable(value), grad = mappable(grad_out);
+  Tensor delta = torch::empty(lse.sizes(), lse.options());
+  agb::PackedArgs a = packed_args(q, k, v, q_offsets, k_offsets, k_lengths, scale);
+  a.out = out.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  agb::PackedGrads g{};
+  g.grad = grad.data_ptr();
+  g.grad_row = row_stride(grad); g.grad_head = head_stride(grad);
+  g.dq = dq.data_ptr(); g.dk = dk.data_ptr(); g.dv = dv.data_ptr();
+  g.delta = delta.data_ptr<float>();
+  check(agb::packed_attention_bwd(a, g, stream_of(q)), "packed_attention_bwd");
+  return {dq, dk, dv};
+}
+
 }  // namespace
 
 void bind_packed(pybind11::module& m) {
   m.def("rotary_embed", &rotary_embed);
   m.def("packed_attention_fwd", &packed_attention_fwd);
+  m.def("packed_attention_bwd", &packed_attention_bwd);
 }
 
 }  // namespace agb_python

@@ -61,4 +61,15 @@ struct PackedArgs {
 };
 cudaError_t packed_attention_tiles(const PackedArgs& args, cudaStream_t stream);
 
+// Gradient: args carries the forward's tensors (out and lse filled in); grad [total_q, hq, dim] with
+// the strides given, dq / dk / dv dense like q / k / v, delta fp32 scratch [hq, total_q].  Rows of no
+// sequence and key rows behind k_lengths receive zeros.
+struct PackedGrads {
+  const void* grad;
+  int64_t grad_row, grad_head;
+  void* dq; void* dk; void* dv;
+  float* delta;
+};
+cudaError_t packed_attention_bwd(const PackedArgs& args, const PackedGrads& grads, cudaStream_t stream);
+
 }  // namespace agb

@@ -1,0 +1,767 @@
+// Gradient of the causal attention over packed sequences, on tcgen05 (bf16 or fp16, heads of up to 128).
+//
+//   p = 2^(s - lse), delta = sum_d dO * O, ds = p (dO v^T - delta)
+//   dq = scale ds k,  dk = scale ds^T q,  dv = p^T dO
+//
+// Two kernels, both without atomics, so a gradient is the same on every run:
+//   packed_dq    one CTA per (128 query rows of a sequence, query head) walks the key tiles up to its
+//                diagonal: S = Q K^T, dP = dO V^T, dQ += dS K.  It also writes delta for
+//   packed_dkdv  one CTA per (128 key rows of a sequence, key head) walks the query tiles that see
+//                them, for the query heads of its group in turn:
+//                S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
+// Shared heads are summed in the accumulators, in FP32.  P and dS are rounded to the tensors' type
+// on their way into the tensor core (scale stays out of dS and is applied to the sums, which keeps
+// small dS of fp16 above its underflow).  Rows of a tile that belong to no one or to another
+// sequence are cleared in shared memory before a product sums over them, so what they hold never
+// spreads.  A tcgen05.mma of 128 rows costs about 90 cycles to issue for up to 128 columns, so both
+// kernels work on whole 128 x 128 blocks and get their overlap from the order of issue.
+#include "agb.h"
+#include "packed.h"
+#include "packed_common.cuh"
+#include "tensormap.h"
+
+namespace agb {
+
+bool make_packed_map(CUtensorMap* map, const void* base, int dim, int heads, int64_t rows, int64_t head_stride,
+                     int64_t row_stride);
+
+namespace {
+
+constexpr int ROWS = 128;
+constexpr int HALF_BYTES = 16384;  // 128 rows x 64 elements
+constexpr int BWD_THREADS = 320;  // 8 elementwise warps, TMA producer, MMA issuer
+constexpr int W_TMA = 8, W_MMA = 9;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct BwdParams {
+  const int* q_offsets; const int* k_offsets; const int* k_lengths;
+  int sequences;
+  int64_t total_q, total_k;
+  const void* out;      // dense [total_q, hq, dim]
+  const void* grad;     // rows and heads at these strides
+  int64_t grad_row, grad_head;
+  const float* lse;     // [hq, total_q]
+  float* delta;         // [hq, total_q]
+  void* dq; void* dk; void* dv;  // dense
+  int hq, hkv, group, dim;
+  float scale, scale_log2;
+  int* status;
+};
+
+// Clears rows [from, 128) of a tile (ATOMS blocks of 128 rows x 128 bytes); converged warp.
+template <int ATOMS>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
+  for (int i = from * 8 + lane; i < ROWS * 8; i += 32)
+    for (int a = 0; a < ATOMS; ++a) *reinterpret_cast<uint4*>(tile + a * HALF_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+template <int ATOMS>
+__device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+  for (int a = 0; a < ATOMS; ++a) tma_load_3d(tile + a * HALF_BYTES, map, bar, a * 64, head, row);
+}
+
+// Writes a warp's 32 rows of an FP32 accumulator, scaled and rounded.  Without `filled` (uniform over
+// the warp) the accumulator holds nothing and zeros are written; so are the rows that are not `live`.
+template <int DP, bool FP16>
+__device__ __forceinline__ void store_rows(uint16_t* dst, uint32_t taddr, int dim, float scale, bool row_ok, bool filled,
+                                           bool live, int c0, int c1) {
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    uint32_t o[32];
+    if (filled) {
+      tmem_ld_32x32(taddr + c * 32, o);
+      tmem_ld_wait();
+    }
+    if (!filled || !live) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0;
+    }
+    if (row_ok) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint4 v;
+        v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]) * scale, __uint_as_float(o[g * 8 + 1]) * scale);
+        v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]) * scale, __uint_as_float(o[g * 8 + 3]) * scale);
+        v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]) * scale, __uint_as_float(o[g * 8 + 5]) * scale);
+        v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]) * scale, __uint_as_float(o[g * 8 + 7]) * scale);
+        if (c * 32 + g * 8 < dim) *reinterpret_cast<uint4*>(dst + c * 32 + g * 8) = v;
+      }
+    }
+  }
+}
+
+template <int DP>
+constexpr int bwd_smem() {  // at least half of an SM's shared memory: two CTAs do not fit in its tensor memory
+  const int bytes = 6 * (DP / 64) * HALF_BYTES + 4 * ROWS * 4 + 1024 + 512;
+  return bytes > 120 * 1024 ? bytes : 120 * 1024;
+}
+
+// ------------------------------------------------------------------------------- dQ
+// Products are issued one tile staggered: S(j+1) = Q K^T | dQ += dS(j) K | dP(j+1) = dO V^T.  The
+// exponentials of tile j+1 run under dQ(j) and dP(j+1), its dS under S(j+2).  Probabilities stay in
+// registers; dS is packed over the first half of the dP columns it came from.
+// TMEM: S[2] [0,256) dP [256,384) dQ [384,512).
+template <int DP, bool FP16>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                 const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 const BwdParams p) {
+  constexpr int ATOMS = DP / 64;
+  constexpr int TILE_BYTES = ATOMS * HALF_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sdO = smem + TILE_BYTES;
+  uint8_t* sK = smem + 2 * TILE_BYTES;
+  uint8_t* sV = smem + 4 * TILE_BYTES;
+  float* halves = reinterpret_cast<float*>(smem + 6 * TILE_BYTES);  // [2][128] parts of delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(halves + 4 * ROWS);
+  uint64_t* q_full = bars;        // Q and dO
+  uint64_t* k_full = bars + 1;    // [2]
+  uint64_t* v_full = bars + 3;    // [2]
+  uint64_t* k_empty = bars + 5;   // [2]
+  uint64_t* v_empty = bars + 7;   // [2]
+  uint64_t* s_full = bars + 9;    // [2] S of a tile is in TMEM
+  uint64_t* dp_full = bars + 11;  // dP of a tile is in TMEM
+  uint64_t* ds_ready = bars + 12; // [2] dS of key chunk c of both halves written over dP (count 8)
+  uint64_t* dq_done = bars + 14;  // every dQ product finished
+  uint64_t* clean = bars + 15;    // rows of the last K and V tile behind the last key cleared
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = int(blockIdx.x % unsigned(p.hq));
+  const int unit = int(blockIdx.x / unsigned(p.hq));
+  const int kv_head = head / p.group;
+  const WaitGuard guard{abort_flag, p.status};
+
+  if (warp == 0) {
+    const PackedSpan span = find_unit(unit, ROWS, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
+                                      p.total_q, p.total_k, head == 0 ? p.status : nullptr);
+    if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
+  }
+  if (warp == 1 && lane == 0) {
+    *abort_flag = 0;
+    mbar_init(q_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(&ds_ready[0], 8);
+    mbar_init(&ds_ready[1], 8);
+    mbar_init(dq_done, 1);
+    mbar_init(clean, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const PackedSpan span = *reinterpret_cast<const PackedSpan*>(span_smem);
+  constexpr uint32_t C_S = 0, C_DP = 256, C_DQ = 384;
+
+  // late tiles of a sequence see the most keys and come first
+  const bool covered = span.unit_in_sequence >= 0 && span.rows > 0;
+  const int first = covered ? ((span.rows + ROWS - 1) / ROWS - 1 - span.unit_in_sequence) * ROWS : 0;
+  const int rows = covered ? min(ROWS, span.rows - first) : 0;
+  const int q_row = span.q0 + first;
+  const int reach = span.keys - span.rows + first;  // row i of the tile sees the keys up to reach + i
+  const int seen_last = covered ? min(span.keys, reach + rows) : 0;
+  const int n_tiles = seen_last > 0 ? (seen_last + ROWS - 1) / ROWS : 0;
+  const int last_valid = span.keys - (n_tiles - 1) * ROWS;
+  const bool ragged = n_tiles > 0 && last_valid < ROWS;
+
+  if (warp == W_TMA) {
+    if (n_tiles > 0) {
+      bool ok = true;
+      if (lane == 0) {
+        mbar_expect_tx(q_full, 2 * TILE_BYTES);
+        load_tile<ATOMS>(sQ, &tm_q, q_full, head, q_row);
+        load_tile<ATOMS>(sdO, &tm_do, q_full, head, q_row);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const int st = j & 1;
+          const uint32_t parity = ((j >> 1) & 1) ^ 1;
+          // the V stage comes free one product earlier than the K stage
+          if (!mbar_wait(&v_empty[st], parity, guard, kTimeoutProducer)) { ok = false; break; }
+          mbar_expect_tx(&v_full[st], TILE_BYTES);
+          load_tile<ATOMS>(sV + st * TILE_BYTES, &tm_v, &v_full[st], kv_head, span.k0 + j * ROWS);
+          if (!mbar_wait(&k_empty[st], parity, guard, kTimeoutProducer)) { ok = false; break; }
+          mbar_expect_tx(&k_full[st], TILE_BYTES);
+          load_tile<ATOMS>(sK + st * TILE_BYTES, &tm_k, &k_full[st], kv_head, span.k0 + j * ROWS);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (ragged && ok) {
+        const int st = (n_tiles - 1) & 1;
+        const uint32_t parity = ((n_tiles - 1) >> 1) & 1;
+        ok = mbar_wait_w(&k_full[st], parity, guard, kTimeoutProducer) &&
+             mbar_wait_w(&v_full[st], parity, guard, kTimeoutProducer);
+        if (ok) {
+          clear_rows<ATOMS>(sK + st * TILE_BYTES, last_valid, lane);
+          clear_rows<ATOMS>(sV + st * TILE_BYTES, last_valid, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(clean);
+        }
+      }
+      if (!ok || *abort_flag) {
+        // give in-flight copies time to land before shared memory is released
+        const uint64_t start = global_timer_ns();
+        while (global_timer_ns() - start < 100000ull) {}
+      }
+    }
+  } else if (warp == W_MMA) {
+    if (n_tiles > 0) {  // the whole warp runs the loop; one elected lane issues
+      constexpr uint32_t idesc_kk = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // both K-major
+      constexpr uint32_t idesc_mn = make_idesc_16(FP16, ROWS, DP, 0, 1);    // B MN-major
+      const uint32_t q_addr = smem_u32(sQ), do_addr = smem_u32(sdO);
+      bool ok = mbar_wait_w(q_full, 0, guard, kTimeoutMma);
+      // S of tile j into buffer j & 1 (its last reader, the exponentials of tile j - 2, finished
+      // before dS(j-2) was announced, which the dQ product of that tile waited for).
+      auto score_s = [&](int j) -> bool {
+        const int st = j & 1;
+        if (!mbar_wait_w(&k_full[st], (j >> 1) & 1, guard, kTimeoutMma)) return false;
+        if (ragged && j == n_tiles - 1 && !mbar_wait_w(clean, 0, guard, kTimeoutMma)) return false;
+        tc_fence_after_sync();
+        const uint32_t k_addr = smem_u32(sK + st * TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+          tc_mma_ss_w(tmem_base + C_S + st * 128, make_smem_desc(q_addr + off, 16, 1024),
+                      make_smem_desc(k_addr + off, 16, 1024), idesc_kk, kk != 0);
+        }
+        tc_commit_w(&s_full[st]);
+        return true;
+      };
+      // dP of tile j over dS(j-1), behind the dQ product that read it.
+      auto score_p = [&](int j) -> bool {
+        const int st = j & 1;
+        if (!mbar_wait_w(&v_full[st], (j >> 1) & 1, guard, kTimeoutMma)) return false;
+        tc_fence_after_sync();
+        const uint32_t v_addr = smem_u32(sV + st * TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+          tc_mma_ss_w(tmem_base + C_DP, make_smem_desc(do_addr + off, 16, 1024),
+                      make_smem_desc(v_addr + off, 16, 1024), idesc_kk, kk != 0);
+        }
+        tc_commit_w(dp_full);
+        tc_commit_w(&v_empty[st]);
+        return true;
+      };
+      if (ok) ok = score_s(0);
+      if (ok) ok = score_p(0);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int st = j & 1;
+        if (j + 1 < n_tiles && !score_s(j + 1)) { ok = false; break; }
+        const uint32_t k_addr = smem_u32(sK + st * TILE_BYTES);
+        // 16 keys per step; the packed columns of the 32 keys [32 g, 32 g + 32) start at column
+        // 32 g.  The warps announce dS in two parts (their first and their second 32 columns:
+        // g = c and g = 2 + c), so half of the product is issued while they finish the rest.
+#pragma unroll
+        for (int c = 0; c < 2 && ok; ++c) {
+          if (!mbar_wait_w(&ds_ready[c], j & 1, guard, kTimeoutMma)) { ok = false; break; }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int s4 = 0; s4 < 4; ++s4) {
+            const int kk = (s4 >> 1) * 4 + c * 2 + (s4 & 1);
+            tc_mma_ts_w(tmem_base + C_DQ, tmem_base + C_DP + (kk >> 1) * 32 + (kk & 1) * 8,
+                        make_smem_desc(k_addr + kk * 2048, HALF_BYTES, 1024), idesc_mn, (j | c | s4) != 0);
+          }
+        }
+        if (!ok) break;
+        tc_commit_w(&k_empty[st]);
+        if (j + 1 < n_tiles && !score_p(j + 1)) { ok = false; break; }
+      }
+      if (ok) tc_commit_w(dq_done);
+    }
+  } else if (warp < 8) {
+    // Warps q and q + 4 share the 32 rows of TMEM lane quarter q and take one half of the 128 key
+    // columns each.
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const int my_row = quarter * 32 + lane;
+    const bool row_ok = my_row < rows;
+    const int64_t stat_index = int64_t(head) * p.total_q + q_row + my_row;
+    // delta of the row: the two halves of its elements, joined through shared memory
+    float part = 0.f;
+    if (row_ok) {
+      const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row + my_row) * p.hq + head) * p.dim;
+      const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row + my_row) * p.grad_row + head * p.grad_head;
+#pragma unroll 4
+      for (int e = half * (DP / 2); e < (half + 1) * (DP / 2); e += 8) {
+        if (e >= p.dim) break;
+        const uint4 a = *reinterpret_cast<const uint4*>(o + e), b = *reinterpret_cast<const uint4*>(g + e);
+        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack16<FP16>(aw[i]), y = unpack16<FP16>(bw[i]);
+          part = fmaf(x.x, y.x, fmaf(x.y, y.y, part));
+        }
+      }
+    }
+    halves[half * ROWS + my_row] = part;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = halves[my_row] + halves[ROWS + my_row];
+    if (row_ok && half == 0) p.delta[stat_index] = delta;
+    const float lse2 = row_ok ? p.lse[stat_index] * LOG2E : 0.f;
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    const float2 nl2 = make_float2(-lse2, -lse2);
+    const float2 nd2 = make_float2(-delta, -delta);
+    const int seen = row_ok ? min(span.keys, reach + my_row + 1) : 0;
+    const int seen_first = rows == ROWS ? min(span.keys, reach + 1) : 0;
+    bool ok = n_tiles > 0;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int buf = j & 1;
+      if (!mbar_wait(&s_full[buf], (j >> 1) & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      tc_fence_after_sync();
+      // only tiles with masked keys or rows pay for the masking; the test is uniform over the CTA
+      const bool plain = seen_first >= (j + 1) * ROWS;
+      const int valid = seen - j * ROWS;
+      float2 prob[32];  // probabilities of this thread's 64 key columns, kept for dS
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sv[32];
+        tmem_ld_32x32(tmem_base + lane_base + C_S + buf * 128 + half * 64 + c * 32, sv);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 x = ffma2(make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sc2, nl2);
+          float2 e = make_float2(exp2f(x.x), exp2f(x.y));
+          if (!plain) {
+            const int col = half * 64 + c * 32 + 2 * i;
+            if (col >= valid) e.x = 0.f;
+            if (col + 1 >= valid) e.y = 0.f;
+          }
+          prob[c * 16 + i] = e;
+        }
+      }
+      if (!mbar_wait(dp_full, j & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dv[32], packed[16];
+        tmem_ld_32x32(tmem_base + lane_base + C_DP + half * 64 + c * 32, dv);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 g = fadd2(make_float2(__uint_as_float(dv[2 * i]), __uint_as_float(dv[2 * i + 1])), nd2);
+          const float2 ds = fmul2(prob[c * 16 + i], g);
+          packed[i] = pack16<FP16>(ds.x, ds.y);
+        }
+        // the packed results land in columns this thread has already read
+        tmem_st_32x16(tmem_base + lane_base + C_DP + half * 64 + c * 32, packed);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_ready[c]);
+      }
+    }
+    if (ok) ok = mbar_wait(dq_done, 0, guard, kTimeoutEpilogue);
+    if (n_tiles == 0 || ok) {
+      tc_fence_after_sync();
+      uint16_t* dst = static_cast<uint16_t*>(p.dq) + (int64_t(q_row + my_row) * p.hq + head) * p.dim;
+      store_rows<DP, FP16>(dst, tmem_base + lane_base + C_DQ, p.dim, p.scale, row_ok, n_tiles > 0, true,
+                           half * (DP / 64), (half + 1) * (DP / 64));
+    }
+    if (span.unit_in_sequence == -2) {  // rows behind the last sequence
+      const int words = p.dim / 8;
+      for (int i = int(threadIdx.x); i < span.rows * words; i += 256) {
+        uint16_t* dst = static_cast<uint16_t*>(p.dq) + ((int64_t(span.q0) + i / words) * p.hq + head) * p.dim + (i % words) * 8;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------- dK / dV
+// Items are (query head of the group, block of 128 query rows that can see the tile), issued
+// dV(i) | S^T(i+1) | dK(i) | dP^T(i+1): the exponentials of item i+1 run under dK(i) and dP^T(i+1), its
+// dS^T under dV(i+1) and S^T(i+2).  Single score buffers: refilling one behind the product that
+// reads its P^T / dS^T is safe, tcgen05.mma operations of one thread execute in issue order.
+// TMEM: S^T [0,128) dP^T [128,256) dV [256,384) dK [384,512).  Warps k and k + 4 share the 32 key
+// rows of lane quarter k and take 64 of the 128 query columns each, 32 at a time; the packed
+// results overwrite the first 16 columns of the 32 they came from.
+template <int DP, bool FP16>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                   const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                   const BwdParams p) {
+  constexpr int ATOMS = DP / 64;
+  constexpr int TILE_BYTES = ATOMS * HALF_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + TILE_BYTES;
+  uint8_t* sQ = smem + 2 * TILE_BYTES;      // [2]
+  uint8_t* sdO = smem + 4 * TILE_BYTES;     // [2]
+  float* stats = reinterpret_cast<float*>(smem + 6 * TILE_BYTES);  // [2][-lse log2(e) [128], -delta [128]]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 4 * ROWS);
+  uint64_t* kv_full = bars;
+  uint64_t* qd_full = bars + 1;     // [2]
+  uint64_t* qd_empty = bars + 3;    // [2]
+  uint64_t* st_full = bars + 5;     // S^T of an item complete
+  uint64_t* dp_full = bars + 6;     // dP^T of an item complete
+  uint64_t* pt_ready = bars + 7;    // [2] P^T of query chunk c of both halves written (count 8)
+  uint64_t* ds_ready = bars + 9;    // dS^T written (count 8)
+  uint64_t* grad_done = bars + 10;  // all gradient products finished
+  uint64_t* stats_bar = bars + 11;  // lse and delta of an item staged (count 256)
+  uint64_t* qd_clean = bars + 12;   // [2] rows of a ragged query block behind the last query cleared
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv_head = int(blockIdx.x % unsigned(p.hkv));
+  const int unit = int(blockIdx.x / unsigned(p.hkv));
+  const WaitGuard guard{abort_flag, p.status};
+
+  if (warp == 0) {
+    const PackedSpan span = find_unit(unit, ROWS, true, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
+                                      p.total_q, p.total_k, kv_head == 0 ? p.status : nullptr);
+    if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
+  }
+  if (warp == 1 && lane == 0) {
+    *abort_flag = 0;
+    mbar_init(kv_full, 1);
+    mbar_init(grad_done, 1);
+    mbar_init(stats_bar, 256);
+    mbar_init(st_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(&pt_ready[0], 8);
+    mbar_init(&pt_ready[1], 8);
+    mbar_init(ds_ready, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&qd_clean[i], 1);
+      mbar_init(&qd_full[i], 1);
+      mbar_init(&qd_empty[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const PackedSpan span = *reinterpret_cast<const PackedSpan*>(span_smem);
+  constexpr uint32_t C_ST = 0, C_DPT = 128, C_DV = 256, C_DK = 384;
+
+  const bool covered = span.unit_in_sequence >= 0;
+  const int k_first = covered ? span.unit_in_sequence * ROWS : 0;
+  const int k_rows = covered ? min(ROWS, span.room - k_first) : 0;       // rows this CTA writes
+  const int k_valid = covered ? max(0, min(ROWS, span.keys - k_first)) : 0;
+  const int shift = span.keys - span.rows;                                // query i sees the keys up to i + shift
+  const int i0 = max(0, k_first - shift);                                 // the first query that sees the tile
+  const int blocks = covered && k_valid > 0 && i0 < span.rows ? (span.rows - i0 + ROWS - 1) / ROWS : 0;
+  const int n_items = blocks * p.group;
+  const int tail_rows = span.rows - i0 - (blocks - 1) * ROWS;             // queries of the last block
+  const bool ragged = blocks > 0 && tail_rows < ROWS;
+
+  if (warp == W_TMA) {
+    if (n_items > 0) {
+      if (lane == 0) {
+        mbar_expect_tx(kv_full, 2 * TILE_BYTES);
+        load_tile<ATOMS>(sK, &tm_k, kv_full, kv_head, span.k0 + k_first);
+        load_tile<ATOMS>(sV, &tm_v, kv_full, kv_head, span.k0 + k_first);
+      }
+      bool ok = true;
+      int head = kv_head * p.group, block = 0;
+      for (int i = 0; i < n_items && ok; ++i) {
+        const int st = i & 1;
+        ok = mbar_wait_w(&qd_empty[st], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(&qd_full[st], 2 * TILE_BYTES);
+          load_tile<ATOMS>(sQ + st * TILE_BYTES, &tm_q, &qd_full[st], head, span.q0 + i0 + block * ROWS);
+          load_tile<ATOMS>(sdO + st * TILE_BYTES, &tm_do, &qd_full[st], head, span.q0 + i0 + block * ROWS);
+        }
+        if (++block == blocks) {
+          block = 0;
+          ++head;
+          // Nothing is lost by waiting here: the stage of item i + 1 comes free with dK(i - 1), which
+          // is issued behind S^T(i).
+          if (ragged) {
+            ok = mbar_wait_w(&qd_full[st], (i >> 1) & 1, guard, kTimeoutProducer);
+            if (!ok) break;
+            clear_rows<ATOMS>(sQ + st * TILE_BYTES, tail_rows, lane);
+            clear_rows<ATOMS>(sdO + st * TILE_BYTES, tail_rows, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&qd_clean[st]);
+          }
+        }
+      }
+      if (!ok || *abort_flag) {
+        const uint64_t start = global_timer_ns();
+        while (global_timer_ns() - start < 100000ull) {}
+      }
+    }
+  } else if (warp == W_MMA) {
+    if (n_items > 0) {  // the whole warp runs the loop; one elected lane issues
+      constexpr uint32_t idesc_s = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // 128 keys x 128 queries
+      constexpr uint32_t idesc_g = make_idesc_16(FP16, ROWS, DP, 0, 1);    // 128 keys x d
+      const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+      uint32_t cleaned = 0;  // bit st: parity of the stage's next cleared block
+      int block = 0;
+      // S^T of item i (needs its Q in shared memory; the buffer's last reader, dV(i-1), was
+      // issued before).
+      auto score_s = [&](int i) -> bool {
+        const int st = i & 1;
+        if (!mbar_wait_w(&qd_full[st], (i >> 1) & 1, guard, kTimeoutMma)) return false;
+        if (++block == blocks) {
+          block = 0;
+          if (ragged) {
+            if (!mbar_wait_w(&qd_clean[st], (cleaned >> st) & 1, guard, kTimeoutMma)) return false;
+            cleaned ^= 1u << st;
+          }
+        }
+        tc_fence_after_sync();
+        const uint32_t q_addr = smem_u32(sQ + st * TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+          tc_mma_ss_w(tmem_base + C_ST, make_smem_desc(k_addr + off, 16, 1024),
+                      make_smem_desc(q_addr + off, 16, 1024), idesc_s, kk != 0);
+        }
+        tc_commit_w(st_full);
+        return true;
+      };
+      // dP^T of item i (its dO arrived with Q; the buffer's last reader, dK(i-1), was issued before).
+      auto score_p = [&](int i) {
+        const uint32_t do_addr = smem_u32(sdO + (i & 1) * TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+          tc_mma_ss_w(tmem_base + C_DPT, make_smem_desc(v_addr + off, 16, 1024),
+                      make_smem_desc(do_addr + off, 16, 1024), idesc_s, kk != 0);
+        }
+        tc_commit_w(dp_full);
+      };
+      bool ok = mbar_wait_w(kv_full, 0, guard, kTimeoutMma);
+      if (ok) ok = score_s(0);
+      if (ok) score_p(0);
+      for (int i = 0; i < n_items && ok; ++i) {
+        const int st = i & 1;
+        const uint32_t q_addr = smem_u32(sQ + st * TILE_BYTES);
+        const uint32_t do_addr = smem_u32(sdO + st * TILE_BYTES);
+        // 16 queries per step; the packed columns of the 32 queries [32 g, 32 g + 32) start at
+        // column 32 g.  The warps announce P^T in two parts (their first and their second 32
+        // columns: g = c and g = 2 + c).
+#pragma unroll
+        for (int c = 0; c < 2 && ok; ++c) {
+          if (!mbar_wait_w(&pt_ready[c], i & 1, guard, kTimeoutMma)) { ok = false; break; }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int s4 = 0; s4 < 4; ++s4) {
+            const int kk = (s4 >> 1) * 4 + c * 2 + (s4 & 1);
+            tc_mma_ts_w(tmem_base + C_DV, tmem_base + C_ST + (kk >> 1) * 32 + (kk & 1) * 8,
+                        make_smem_desc(do_addr + kk * 2048, HALF_BYTES, 1024), idesc_g, (i | c | s4) != 0);
+          }
+        }
+        if (!ok) break;
+        if (i + 1 < n_items && !score_s(i + 1)) { ok = false; break; }
+        if (!mbar_wait_w(ds_ready, i & 1, guard, kTimeoutMma)) { ok = false; break; }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int kk = 0; kk < ROWS / 16; ++kk)
+          tc_mma_ts_w(tmem_base + C_DK, tmem_base + C_DPT + (kk >> 1) * 32 + (kk & 1) * 8,
+                      make_smem_desc(q_addr + kk * 2048, HALF_BYTES, 1024), idesc_g, (i | kk) != 0);
+        tc_commit_w(&qd_empty[st]);
+        if (i + 1 < n_items) score_p(i + 1);
+      }
+      if (ok) tc_commit_w(grad_done);
+    }
+  } else if (warp < 8) {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const int tid = (warp << 5) + lane;      // 0..255
+    const int key = quarter * 32 + lane;     // key row of this thread
+    bool ok = n_items > 0;
+    // Per query column the warps need -lse*log2(e) and -delta.  They are staged in shared memory one
+    // item ahead: the global loads of item i + 1 are issued before the work on item i and stored
+    // behind it, so their latency never sits between two items.
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    auto fetch_stat = [&](int g, int block) -> float {
+      // threads 0..127: -lse*log2(e) (or -inf: probability 0), threads 128..255: -delta
+      const int col = i0 + block * ROWS + (tid & (ROWS - 1));
+      const bool valid = col < span.rows;
+      const int64_t at = int64_t(kv_head * p.group + g) * p.total_q + span.q0 + col;
+      if (tid < ROWS) return valid ? -p.lse[at] * LOG2E : -INFINITY;
+      return valid ? -p.delta[at] : 0.f;
+    };
+    if (ok) {
+      stats[tid] = fetch_stat(0, 0);
+      mbar_arrive(stats_bar);
+    }
+    int g = 0, block = 0;
+    for (int i = 0; i < n_items && ok; ++i) {
+      const bool more = i + 1 < n_items;
+      const int q_first = i0 + block * ROWS;
+      const int q_rows = min(ROWS, span.rows - q_first);
+      if (++block == blocks) { block = 0; ++g; }
+      float next_stat = 0.f;
+      if (more) next_stat = fetch_stat(g, block);
+      const float* my_stats = stats + (i & 1) * 2 * ROWS + half * 64;
+      // query column c sees this key where c >= from, of the block's q_rows; only blocks that mask
+      // pay for it, and the test is uniform over the CTA
+      const int from = key < k_valid ? k_first + key - shift - q_first : ROWS;
+      const bool plain = k_valid == ROWS && q_rows == ROWS && k_first + ROWS - 1 - shift <= q_first;
+      if (!mbar_wait(stats_bar, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      if (!mbar_wait(st_full, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      tc_fence_after_sync();
+      float2 prob[32];  // the probabilities of this thread's 64 query columns, kept for dS^T
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sv[32], pp[16];
+        tmem_ld_32x32(tmem_base + lane_base + C_ST + half * 64 + c * 32, sv);
+        tmem_ld_wait();
+        const float4* nl4 = reinterpret_cast<const float4*>(my_stats + c * 32);
+#pragma unroll
+        for (int k4 = 0; k4 < 8; ++k4) {  // four query columns per step
+          const float4 nl = nl4[k4];
+          const float2 x0 = ffma2(make_float2(__uint_as_float(sv[4 * k4]), __uint_as_float(sv[4 * k4 + 1])), sc2,
+                                  make_float2(nl.x, nl.y));
+          const float2 x1 = ffma2(make_float2(__uint_as_float(sv[4 * k4 + 2]), __uint_as_float(sv[4 * k4 + 3])), sc2,
+                                  make_float2(nl.z, nl.w));
+          float2 e0 = make_float2(exp2f(x0.x), exp2f(x0.y));
+          float2 e1 = make_float2(exp2f(x1.x), exp2f(x1.y));
+          if (!plain) {
+            const int col = half * 64 + c * 32 + 4 * k4;
+            if (col < from || col >= q_rows) e0.x = 0.f;
+            if (col + 1 < from || col + 1 >= q_rows) e0.y = 0.f;
+            if (col + 2 < from || col + 2 >= q_rows) e1.x = 0.f;
+            if (col + 3 < from || col + 3 >= q_rows) e1.y = 0.f;
+          }
+          prob[c * 16 + 2 * k4] = e0;
+          prob[c * 16 + 2 * k4 + 1] = e1;
+          pp[2 * k4] = pack16<FP16>(e0.x, e0.y);
+          pp[2 * k4 + 1] = pack16<FP16>(e1.x, e1.y);
+        }
+        // the packed results land in columns this thread has already read
+        tmem_st_32x16(tmem_base + lane_base + C_ST + half * 64 + c * 32, pp);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pt_ready[c]);
+      }
+      if (!mbar_wait(dp_full, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dv[32], dd[16];
+        tmem_ld_32x32(tmem_base + lane_base + C_DPT + half * 64 + c * 32, dv);
+        tmem_ld_wait();
+        const float4* nd4 = reinterpret_cast<const float4*>(my_stats + ROWS + c * 32);
+#pragma unroll
+        for (int k4 = 0; k4 < 8; ++k4) {
+          const float4 nd = nd4[k4];
+          const float2 g0 = fadd2(make_float2(__uint_as_float(dv[4 * k4]), __uint_as_float(dv[4 * k4 + 1])),
+                                  make_float2(nd.x, nd.y));
+          const float2 g1 = fadd2(make_float2(__uint_as_float(dv[4 * k4 + 2]), __uint_as_float(dv[4 * k4 + 3])),
+                                  make_float2(nd.z, nd.w));
+          const float2 d0 = fmul2(prob[c * 16 + 2 * k4], g0), d1 = fmul2(prob[c * 16 + 2 * k4 + 1], g1);
+          dd[2 * k4] = pack16<FP16>(d0.x, d0.y);
+          dd[2 * k4 + 1] = pack16<FP16>(d1.x, d1.y);
+        }
+        tmem_st_32x16(tmem_base + lane_base + C_DPT + half * 64 + c * 32, dd);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+      // The other stats buffer was last read for item i - 1; every thread has passed the wait
+      // of phase i above, which all threads entered only after finishing item i - 1.
+      if (more) {
+        stats[((i + 1) & 1) * 2 * ROWS + tid] = next_stat;
+        mbar_arrive(stats_bar);
+      }
+    }
+    if (ok) ok = mbar_wait(grad_done, 0, guard, kTimeoutEpilogue);
+    if (n_items == 0 || ok) {
+      tc_fence_after_sync();
+      // the two halves write one gradient each
+      uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) +
+                      (int64_t(span.k0 + k_first + key) * p.hkv + kv_head) * p.dim;
+      // rows that are no keys (the room behind them) get zeros
+      store_rows<DP, FP16>(dst, tmem_base + lane_base + (half == 0 ? C_DV : C_DK), p.dim, half == 0 ? 1.f : p.scale,
+                           key < k_rows, n_items > 0, key < k_valid, 0, DP / 32);
+    }
+    if (span.unit_in_sequence == -2) {  // rows behind the last sequence
+      const int words = p.dim / 8;
+      for (int i = tid; i < span.rows * words; i += 256) {
+        const int64_t at = ((int64_t(span.k0) + i / words) * p.hkv + kv_head) * p.dim + (i % words) * 8;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dk) + at) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dv) + at) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int DP, bool FP16>
+cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap& tdo, const CUtensorMap& tk,
+                   const CUtensorMap& tv, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(packed_dq_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       bwd_smem<DP>());
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(packed_dkdv_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<DP>());
+  if (e != cudaSuccess) return e;
+  const int64_t q_grid = (p.total_q / ROWS + p.sequences + 1) * p.hq;
+  const int64_t k_grid = (p.total_k / ROWS + p.sequences + 1) * p.hkv;
+  if (q_grid > 2147483647ll || k_grid > 2147483647ll) {
+    set_error_detail("packed_attention: too many tiles for one launch");
+    return cudaErrorInvalidValue;
+  }
+  packed_dq_kernel<DP, FP16><<<unsigned(q_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
+  packed_dkdv_kernel<DP, FP16><<<unsigned(k_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t packed_attention_bwd(const PackedArgs& a, const PackedGrads& g, cudaStream_t stream) {
+  CUtensorMap tq, tdo, tk, tv;
+  if (!make_packed_map(&tq, a.q, a.dim, a.hq, a.total_q, a.q_head, a.q_row) ||
+      !make_packed_map(&tdo, g.grad, a.dim, a.hq, a.total_q, g.grad_head, g.grad_row) ||
+      !make_packed_map(&tk, a.k, a.dim, a.hkv, a.total_k, a.k_head, a.k_row) ||
+      !make_packed_map(&tv, a.v, a.dim, a.hkv, a.total_k, a.v_head, a.v_row))
+    return cudaErrorInvalidValue;
+  BwdParams p{};
+  p.q_offsets = a.q_offsets; p.k_offsets = a.k_offsets; p.k_lengths = a.k_lengths;
+  p.sequences = a.sequences;
+  p.total_q = a.total_q; p.total_k = a.total_k;
+  p.out = a.out; p.grad = g.grad; p.grad_row = g.grad_row; p.grad_head = g.grad_head;
+  p.lse = a.lse; p.delta = g.delta;
+  p.dq = g.dq; p.dk = g.dk; p.dv = g.dv;
+  p.hq = a.hq; p.hkv = a.hkv; p.group = a.hq / a.hkv; p.dim = a.dim;
+  p.scale = a.scale; p.scale_log2 = a.scale * LOG2E;
+  p.status = a.status;
+  if (a.dim <= 64)
+    return a.fp16 ? launch<64, true>(p, tq, tdo, tk, tv, stream) : launch<64, false>(p, tq, tdo, tk, tv, stream);
+  return a.fp16 ? launch<128, true>(p, tq, tdo, tk, tv, stream) : launch<128, false>(p, tq, tdo, tk, tv, stream);
+}
+
+}  // namespace agb

@@ -174,6 +174,25 @@ def rotary_embed(query: torch.Tensor, key: torch.Tensor | None, positions: torch
 
 
 # ---------------------------------------------------------------------------- packed attention
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, q_offsets, k_offsets, k_lengths, scale):
+        native.count()
+        out, lse = native.ext().packed_attention_fwd(query, key, value, q_offsets, k_offsets, k_lengths, scale, True)
+        ctx.save_for_backward(query, key, value, out, lse, q_offsets, k_offsets, k_lengths)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        query, key, value, out, lse, q_offsets, k_offsets, k_lengths = ctx.saved_tensors
+        native.count(2)
+        grads = native.ext().packed_attention_bwd(grad, query, key, value, out, lse, q_offsets, k_offsets, k_lengths,
+                                                  ctx.scale)
+        return *grads, None, None, None, None
+
+
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_offsets: torch.Tensor,
                      k_offsets: torch.Tensor | None = None, *, k_lengths: torch.Tensor | None = None,
                      scale: float | None = None) -> torch.Tensor:
@@ -225,4 +244,5 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)):
             native.count()
             return native.ext().packed_attention_fwd(query, key, value, q_offsets, k_offsets, k_lengths, scale, False)[0]
+        return _PackedAttention.apply(query, key, value, q_offsets, k_offsets, k_lengths, scale)
     return reference.packed_attention(query, key, value, q_offsets, k_offsets, k_lengths, scale)

@@ -243,3 +243,77 @@ def test_attention_reports_bad_offsets(rows):
         ops.packed_attention(q, k, v, given["q_offsets"], given["k_offsets"], k_lengths=given["k_lengths"])
         assert _status() == 7, bad
         native.ext().status(torch.cuda.current_device()).zero_()
+
+
+# ------------------------------------------------------------------------------------ gradients
+def _check_gradients(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw):
+    q, k, v, qo, ko, kl, spans = _case(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw)
+    g = torch.Generator(device=DEV).manual_seed(77)
+    grad = torch.randn(q.shape, device=DEV, generator=g).to(dtype)
+    grad[sum(q_lengths):] = float("nan")  # rows of no sequence
+    for t in (q, k, v):
+        t.requires_grad_()
+    before = native.launches()
+    out = ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    grads = torch.autograd.grad(out, (q, k, v), grad)
+    assert native.launches() > before + 1
+    assert _status() == 0
+    want = oracle.attention(q.detach(), k.detach(), v.detach(), spans, dim ** -0.5, grad)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        oracle.assert_close(got, *want[name], name)
+    for got, used in zip((out, *grads), (want["out"], want["dq"], want["dk"], want["dv"])):
+        untouched = used[1].flatten(1).sum(-1) == 0  # rows of no sequence, room behind the keys
+        assert not got[untouched].any()
+    return q, k, v, qo, ko, kl, out, grad, grads
+
+
+@pytest.mark.parametrize("lengths", PROMPTS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (8, 1)])
+def test_gradients_of_prompts(lengths, heads, kv_heads):
+    _check_gradients(lengths, lengths, heads, kv_heads, 128, BF16, behind=150)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [8, 40, 64, 72, 96, 128])
+def test_gradients_of_head_sizes_and_types(dim, dtype):
+    _check_gradients([130, 3, 200], [130, 3, 200], 4, 2, dim, dtype)
+
+
+@pytest.mark.parametrize("q_lengths,k_lengths", [([5, 100], [700, 333]), ([129, 1, 64], [129, 900, 70]),
+                                                  ([50, 140, 10, 4], [20, 100, 0, 3]), ([64, 3], [0, 0]), ([260], [128])])
+def test_gradients_of_continued_prompts(q_lengths, k_lengths):
+    _check_gradients(q_lengths, k_lengths, 4, 2, 128, BF16, room=13, behind=2)
+
+
+def test_gradients_repeat_bit_for_bit_and_take_any_layout():
+    q, k, v, qo, ko, kl, out, grad, grads = _check_gradients([130, 70], [130, 70], 4, 2, 64, BF16)
+    again = ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+    head_major = grad.transpose(0, 1).contiguous().transpose(0, 1)
+    for a, b in zip(grads, torch.autograd.grad(again, (q, k, v), head_major)):
+        assert torch.equal(a, b)
+    # a broadcast gradient, and only one leaf
+    again = ops.packed_attention(q, k.detach(), v.detach(), qo, ko, k_lengths=kl)
+    (got,) = torch.autograd.grad(again.sum(), (q,))
+    want = oracle.attention(q.detach(), k.detach(), v.detach(), [(0, 130, 0, 130), (130, 70, 130, 70)], 0.125,
+                            torch.ones_like(q))
+    oracle.assert_close(got, *want["dq"])
+
+
+def test_gradient_against_differences():
+    """The directional derivative of a smooth function of the output, in a direction of all inputs."""
+    q, k, v, qo, ko, kl, spans = _case([40, 90], [40, 90], 4, 2, 64, FP16, seed=3)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    weight = torch.randn(q.shape, device=DEV, generator=g).to(FP16)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.packed_attention(*leaves, qo), leaves, weight)
+    steps = [torch.randn(t.shape, device=DEV, generator=g).double() for t in (q, k, v)]
+    slope = sum((a.double() * b).sum() for a, b in zip(grads, steps))
+    h = 1e-5
+
+    def value(sign):
+        moved = [t.double() + sign * h * s for t, s in zip((q, k, v), steps)]
+        return (oracle.attention(*moved, spans, 0.125)["out"][0] * weight.double()).sum()
+
+    want = oracle.attention(q, k, v, spans, 0.125, weight)
+    allowed = sum((want[n][1] * s.abs()).sum() for n, s in zip(("dq", "dk", "dv"), steps))
+    assert abs(slope - (value(1) - value(-1)) / (2 * h)) <= allowed + 1e-6 * abs(slope) + 1e-3
