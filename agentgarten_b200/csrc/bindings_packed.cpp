@@ -3,6 +3,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "agb.h"
 #include "bindings.h"
 #include "packed.h"
@@ -105,6 +108,45 @@ agb::PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, c
   return a;
 }
 
+// The kernels are chosen by the totals alone: the lengths are on the device.
+//
+// The few-row kernel where the sequences have on average no more rows than one of its products.
+bool few_rows(const agb::PackedArgs& a) {
+  const int heads = std::min(a.hq / a.hkv, 16);
+  return a.total_q * heads <= int64_t(16) * a.sequences;
+}
+
+// Keys of a chunk: about three CTAs for every place (two on an SM), and never so few that joining them shows.
+int rows_chunk(const agb::PackedArgs& a, int sms) {
+  const int64_t work = a.total_k * a.hkv * agb::packed_rows_pieces(a.hq / a.hkv);
+  const int64_t chunk = (work / (int64_t(sms) * 2 * 3) + 63) / 64 * 64;
+  return int(std::min<int64_t>(std::max<int64_t>(chunk, 256), 8192));
+}
+
+// Key ranges of a tile: the count that makes the estimated launch shortest.  In units of one key
+// tile's work (about 0.9 us): the longest CTA, twice the mean's, or all of the work over the SMs;
+// then the join, about 4 us and the partial results' way to memory and back.
+int tile_splits(const agb::PackedArgs& a, int sms) {
+  const bool paired = (a.hq / a.hkv) % 2 == 0;
+  const double step = paired ? 128 : 256;
+  const double rows = double(a.total_q) / a.sequences, keys = double(a.total_k) / a.sequences;
+  const double pieces = std::ceil(rows / step);
+  const double seen = std::max(keys - rows / 2, rows / 2);  // of a row, on average
+  const double tiles = std::ceil(seen / 128);
+  const double all = a.sequences * pieces * (paired ? a.hq / 2 : a.hq) * tiles / sms;
+  const double partial = double(a.total_q) * a.hq * a.dim * 8 / 6.5e6 / 0.9;
+  int best = 1;
+  double best_cost = std::max(2 * tiles, all);
+  for (int s = 2; s <= 16 && 2 * tiles / s >= 4; ++s) {
+    const double cost = std::max(std::ceil(2 * tiles / s), all) + 4 / 0.9 + s * partial;
+    if (cost < 0.9 * best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
 // (out, lse [hq, total_q] or an empty tensor)
 std::tuple<Tensor, Tensor> packed_attention_fwd(const Tensor& query, const Tensor& key, const Tensor& value,
                                                 const Tensor& q_offsets, const Tensor& k_offsets,
@@ -123,6 +165,28 @@ std::tuple<Tensor, Tensor> packed_attention_fwd(const Tensor& query, const Tenso
   agb::PackedArgs a = packed_args(q, k, v, q_offsets, k_offsets, k_lengths, scale);
   a.out = out.data_ptr();
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  Tensor part_out, part_lse;
+  const int sms = sm_count(q), group = a.hq / a.hkv;
+  if (few_rows(a)) {
+    const int64_t pieces = agb::packed_rows_pieces(group);
+    a.chunk = rows_chunk(a, sms);
+    if (a.total_k > a.chunk) {
+      const int64_t slots = (a.total_k / a.chunk + a.sequences) * a.hkv * pieces * 16;
+      part_out = torch::empty({slots, a.dim}, fp32);
+      part_lse = torch::empty({slots}, fp32);
+      a.part_out = part_out.data_ptr<float>();
+      a.part_lse = part_lse.data_ptr<float>();
+    }
+    check(agb::packed_attention_rows(a, stream_of(q)), "packed_attention");
+    return {out, lse};
+  }
+  a.splits = tile_splits(a, sms);
+  if (a.splits > 1) {
+    part_out = torch::empty({a.splits, a.total_q, a.hq, a.dim}, fp32);
+    part_lse = torch::empty({a.splits, a.total_q, a.hq}, fp32);
+    a.part_out = part_out.data_ptr<float>();
+    a.part_lse = part_lse.data_ptr<float>();
+  }
   check(agb::packed_attention_tiles(a, stream_of(q)), "packed_attention");
   return {out, lse};
 }

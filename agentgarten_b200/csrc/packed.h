@@ -52,14 +52,18 @@ struct PackedArgs {
   int hq, hkv, dim, fp16;
   float scale;
   int* status;
-  // Key splits of the tile kernel (1: none) and its FP32 partial results [splits, total_q, hq, dim],
-  // [splits, hq, total_q]; the few-row kernel has chunks of `chunk` keys instead and partial
-  // results [units, pieces, rows, dim], [units, pieces, rows] with units = total_k / chunk + sequences.
+  // FP32 partial results of the keys' ranges: with splits > 1 the tile kernel's [splits, total_q, hq, dim]
+  // and [splits, total_q, hq]; for the few-row kernel, whose ranges are chunks of `chunk` keys,
+  // [units, hkv, pieces, 16, dim] and [units, hkv, pieces, 16] with units = total_k / chunk + sequences
+  // and pieces = packed_rows_pieces(hq / hkv) (unused when total_k <= chunk).
   int splits, chunk;
   float* part_out;
   float* part_lse;
 };
 cudaError_t packed_attention_tiles(const PackedArgs& args, cudaStream_t stream);
+// The same function for sequences of few query rows; any number of rows is right.
+cudaError_t packed_attention_rows(const PackedArgs& args, cudaStream_t stream);
+int packed_rows_pieces(int group);
 
 // Gradient: args carries the forward's tensors (out and lse filled in); grad [total_q, hq, dim] with
 // the strides given, dq / dk / dv dense like q / k / v, delta fp32 scratch [hq, total_q].  Rows of no

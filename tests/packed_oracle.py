@@ -1,7 +1,8 @@
 """Plain 64-bit definitions of the packed operators, with the error that rounding may leave.
 
 ``eps`` below is the unit roundoff of the tensors' type: a rounding is off by at most ``eps`` of the
-value.  32-bit arithmetic adds less than ``SLACK`` of the same sums (accumulations of up to a few
+value, or, below the type's smallest normal number, by half of its constant spacing, which is ``eps``
+of that number (2^-25 in fp16).  32-bit arithmetic adds less than ``SLACK`` of the same sums (accumulations of up to a few
 thousand terms at 2^-24 each, the exponential's and the scores' last bits).
 """
 
@@ -14,6 +15,10 @@ SLACK = 1e-4
 
 def unit(dtype):
     return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    return unit(dtype) * torch.finfo(dtype).smallest_normal
 
 
 def rotary(x, positions, inverse, amplitude=1.0, axis=None, interleaved=False):
@@ -31,7 +36,7 @@ def rotary(x, positions, inverse, amplitude=1.0, axis=None, interleaved=False):
     # by at most 2 units of 2^-24, amplitude, product and sum by one each: 10 units in all.
     size = torch.zeros_like(out)
     size[..., first] = size[..., second] = a.abs() + b.abs()
-    bound = unit(x.dtype) * out.abs() + 10 * 2.0 ** -24 * amplitude * size
+    bound = unit(x.dtype) * out.abs() + tiny(x.dtype) + 10 * 2.0 ** -24 * amplitude * size
     if x.dtype == torch.float32:  # the rounding to the type is the sum's own, counted above
         bound = 10 * 2.0 ** -24 * amplitude * size
     return out, bound
@@ -44,7 +49,7 @@ def attention(q, k, v, spans, scale, grad=None):
     The kernels round p and ds to the type before a product, and every result once; delta is taken
     from the rounded out.
     """
-    eps, group = unit(q.dtype), q.shape[1] // k.shape[1]
+    eps, group, least = unit(q.dtype), q.shape[1] // k.shape[1], tiny(q.dtype)
 
     def zeros(t):
         return torch.zeros(t.shape, dtype=torch.float64, device=t.device)
@@ -64,7 +69,8 @@ def attention(q, k, v, spans, scale, grad=None):
             p = torch.softmax(s, -1)
             p[~some] = 0
             o = p @ V
-            o_err = eps * (p @ V.abs()) + eps * o.abs() + SLACK * (p @ V.abs())
+            # p is rounded before it is divided by its sum, which is at least 1
+            o_err = (eps + SLACK) * (p @ V.abs()) + eps * o.abs() + least * (1 + seen.double() @ V.abs())
             res["out"][0][q0:q0 + rows, h] = o
             res["out"][1][q0:q0 + rows, h] = o_err
             if grad is None:
@@ -73,17 +79,17 @@ def attention(q, k, v, spans, scale, grad=None):
             delta = (dO * o).sum(-1, keepdim=True)
             ds = p * (dO @ V.t() - delta)
             size = p * (dO.abs() @ V.abs().t() + (dO * o).abs().sum(-1, keepdim=True))
-            ds_err = eps * ds.abs() + p * (dO.abs() * o_err).sum(-1, keepdim=True) + SLACK * size
+            ds_err = eps * ds.abs() + least * seen + p * (dO.abs() * o_err).sum(-1, keepdim=True) + SLACK * size
             rows_, keys_ = slice(q0, q0 + rows), slice(k0, k0 + keys)
             for name, at, head, value, error in (
                     ("dq", rows_, h, scale * ds @ K, scale * ds_err @ K.abs()),
                     ("dk", keys_, g, scale * ds.t() @ Q, scale * ds_err.t() @ Q.abs()),
-                    ("dv", keys_, g, p.t() @ dO, (eps + SLACK) * (p.t() @ dO.abs()))):
+                    ("dv", keys_, g, p.t() @ dO, ((eps + SLACK) * p + least * seen).t() @ dO.abs())):
                 res[name][0][at, head] += value
                 res[name][1][at, head] += error
     for name, (value, bound) in res.items():
         if name != "out":
-            bound += eps * value.abs()
+            bound += eps * value.abs() + least * (bound > 0)
     return res
 
 

@@ -167,6 +167,14 @@ def test_attention_of_continued_prompts(q_lengths, k_lengths, heads, kv_heads):
     _check_forward(q_lengths, k_lengths, heads, kv_heads, 128, BF16, room=13, behind=300)
 
 
+@pytest.mark.parametrize("q_lengths,k_lengths", [([40, 200], [5001, 3000]), ([33], [20000]), ([100, 30, 70], [90, 8000, 1])])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 1)])
+def test_attention_over_split_key_ranges(q_lengths, k_lengths, heads, kv_heads):
+    """Few tiles against many keys: ranges of keys side by side, joined by a second launch."""
+    _check_forward(q_lengths, k_lengths, heads, kv_heads, 72, BF16, room=3, behind=260)
+    _check_gradients(q_lengths, k_lengths, heads, kv_heads, 72, FP16, room=3, behind=1)
+
+
 @pytest.mark.parametrize("k_lengths", [[1], [15, 16, 17, 31], [100, 0, 1, 2049], [5000], [257] * 40])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 4, 64), (32, 1, 96), (40, 2, 80)])
 def test_attention_of_single_tokens(k_lengths, heads, kv_heads, dim):
