@@ -77,4 +77,5 @@ def count(n: int = 1) -> None:
 
 
 def launches() -> int:
-    return _launches
+    # the packed operators launch, and count, from C++
+    return _launches + (_ext.packed_launches() if _ext is not None else 0)

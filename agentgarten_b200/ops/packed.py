@@ -25,11 +25,11 @@ from dataclasses import dataclass
 import torch
 
 from . import native, reference
-from .pointwise import _plain
 
 __all__ = ["RotaryFrequencies", "packed_attention", "rotary_embed", "rotary_frequencies"]
 
 SCALINGS = ("linear", "ntk", "yarn")
+_KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 # ------------------------------------------------------------------------------- rotary positions
@@ -105,37 +105,6 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10_000.0, *, scaling: str
     return RotaryFrequencies((inverse / (2 * math.pi)).to(device), amplitude, axis)
 
 
-def _turn(query, key, positions, frequencies: RotaryFrequencies, interleaved: bool, backwards: bool):
-    native.count()
-    out = native.ext().rotary_embed(query, key, positions, frequencies.turns, frequencies.axis,
-                                    frequencies.amplitude, interleaved, backwards)
-    return out[0], (out[1] if key is not None else None)
-
-
-class _RotaryEmbed(torch.autograd.Function):
-    """The gradient of a turn is the turn back: nothing of the values is kept."""
-
-    @staticmethod
-    def forward(ctx, query, key, positions, frequencies, interleaved):
-        ctx.save_for_backward(positions)
-        ctx.frequencies, ctx.interleaved = frequencies, interleaved
-        ctx.set_materialize_grads(False)
-        return _turn(query, key, positions, frequencies, interleaved, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dquery, dkey):
-        (positions,) = ctx.saved_tensors
-        present = [g for g in (dquery, dkey) if g is not None]
-        grads = [None, None]
-        if len(present) == 2:
-            grads = list(_turn(*present, positions, ctx.frequencies, ctx.interleaved, True))
-        elif present:
-            grads[0 if dquery is not None else 1] = _turn(
-                present[0], None, positions, ctx.frequencies, ctx.interleaved, True)[0]
-        return grads[0], grads[1], None, None, None
-
-
 def rotary_embed(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
                  frequencies: RotaryFrequencies, *, interleaved: bool = False):
     """Query and key turned by their positions, in one pass: ``(query, key)`` as new tensors.
@@ -148,51 +117,32 @@ def rotary_embed(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     are exact for any position that the type of ``positions`` holds; the turn is 32-bit arithmetic,
     rounded once.  Differentiable in query and key.
     """
+    f = frequencies
+    if query.is_cuda and native.use(query, dtypes=_KERNEL_TYPES):
+        out = native.ext().rotary_embed(query, key, positions, f.turns, f.axis, f.amplitude, interleaved)
+        if out is not None:
+            return out[0], (out[1] if key is not None else None)
     given = [query] if key is None else [query, key]
     lead = query.shape[:-2]
     for name, t in zip(("query", "key"), given):
         if t.dim() < 3 or t.shape[:-2] != lead or t.shape[-1] != query.shape[-1] or t.shape[-2] == 0:
             raise ValueError(f"rotary_embed: {name} {tuple(t.shape)} is not [..., heads, dim] over {tuple(lead)}")
-        if t.dtype != query.dtype or t.dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float64):
+        if t.dtype != query.dtype or t.dtype not in (*_KERNEL_TYPES, torch.float64):
             raise TypeError(f"rotary_embed: {name} is {t.dtype}: both are bf16, fp16, fp32 or fp64")
-    if frequencies.rotary_dim > query.shape[-1]:
-        raise ValueError(f"rotary_embed: {frequencies.rotary_dim} elements to turn in heads of {query.shape[-1]}")
-    want = tuple(lead) if frequencies.axis is None else (*lead, 3)
+    if f.rotary_dim > query.shape[-1]:
+        raise ValueError(f"rotary_embed: {f.rotary_dim} elements to turn in heads of {query.shape[-1]}")
+    want = tuple(lead) if f.axis is None else (*lead, 3)
     if tuple(positions.shape) != want:
         raise ValueError(f"rotary_embed: positions {tuple(positions.shape)} are not {want}")
     if positions.dtype not in (torch.int32, torch.int64, torch.float32):
         raise TypeError(f"rotary_embed: positions are int32, int64 or fp32, not {positions.dtype}")
-    if any(t.device != query.device for t in (*given, positions, frequencies.turns)):
+    if any(t.device != query.device for t in (*given, positions, f.turns)):
         raise ValueError("rotary_embed: query, key, positions and frequencies are on one device")
-    if native.use(query, dtypes=(torch.bfloat16, torch.float16, torch.float32)) and _plain(*given):
-        if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-            return _RotaryEmbed.apply(query, key, positions, frequencies, interleaved)
-        return _turn(query, key, positions, frequencies, interleaved, False)
-    turned = [reference.rotary_embed(t, positions, frequencies.turns, frequencies.amplitude, frequencies.axis,
-                                     interleaved) for t in given]
+    turned = [reference.rotary_embed(t, positions, f.turns, f.amplitude, f.axis, interleaved) for t in given]
     return turned[0], (turned[1] if key is not None else None)
 
 
 # ---------------------------------------------------------------------------- packed attention
-class _PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, query, key, value, q_offsets, k_offsets, k_lengths, scale):
-        native.count()
-        out, lse = native.ext().packed_attention_fwd(query, key, value, q_offsets, k_offsets, k_lengths, scale, True)
-        ctx.save_for_backward(query, key, value, out, lse, q_offsets, k_offsets, k_lengths)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        query, key, value, out, lse, q_offsets, k_offsets, k_lengths = ctx.saved_tensors
-        native.count(2)
-        grads = native.ext().packed_attention_bwd(grad, query, key, value, out, lse, q_offsets, k_offsets, k_lengths,
-                                                  ctx.scale)
-        return *grads, None, None, None, None
-
-
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_offsets: torch.Tensor,
                      k_offsets: torch.Tensor | None = None, *, k_lengths: torch.Tensor | None = None,
                      scale: float | None = None) -> torch.Tensor:
@@ -213,6 +163,10 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     Differentiable in query, key and value.  Scores, statistics and sums are FP32; probabilities
     are rounded to the tensors' type where they enter a matrix product.
     """
+    if query.is_cuda and native.use(query, dtypes=_KERNEL_TYPES[:2]):
+        out = native.ext().packed_attention(query, key, value, q_offsets, k_offsets, k_lengths, scale)
+        if out is not None:
+            return out
     if query.dim() != 3 or key.dim() != 3 or value.shape != key.shape or query.shape[-1] != key.shape[-1]:
         raise ValueError(f"packed_attention: query {tuple(query.shape)}, key {tuple(key.shape)} and value "
                          f"{tuple(value.shape)} are not [total, heads, dim] with one dim")
@@ -239,10 +193,4 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise ValueError("packed_attention: scale is positive")
-    if (native.use(query, dtypes=(torch.bfloat16, torch.float16)) and dim % 8 == 0 and dim <= 128
-            and _plain(query, key, value)):
-        if not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)):
-            native.count()
-            return native.ext().packed_attention_fwd(query, key, value, q_offsets, k_offsets, k_lengths, scale, False)[0]
-        return _PackedAttention.apply(query, key, value, q_offsets, k_offsets, k_lengths, scale)
     return reference.packed_attention(query, key, value, q_offsets, k_offsets, k_lengths, scale)

@@ -76,6 +76,9 @@ def test_rotary_strides():
     x = torch.randn(4, 6, 2, 64, device=DEV, generator=g)[::2, ::3]
     at = torch.arange(4, device=DEV).view(2, 2)
     oracle.assert_close(ops.rotary_embed(x, None, at, f)[0], *oracle.rotary(x, at, inverse))
+    x = torch.randn(4, 1, 2, 64, device=DEV, generator=g).expand(4, 3, 2, 64)
+    at = torch.arange(12, device=DEV).view(4, 3)
+    oracle.assert_close(ops.rotary_embed(x, None, at, f)[0], *oracle.rotary(x, at, inverse))
     empty = torch.randn(0, 4, 64, device=DEV)
     assert ops.rotary_embed(empty, empty, positions[:0], f)[1].shape == empty.shape
 
@@ -97,9 +100,16 @@ def test_rotary_gradients(dtype, interleaved):
     oracle.assert_close(got, *oracle.rotary(torch.ones_like(k), at, -inverse, f.amplitude, interleaved=interleaved))
 
 
-def test_rotary_device_and_type_refusals():
-    q = torch.randn(4, 2, 64, device=DEV)
+def test_rotary_refusals():
+    q, k, at = torch.randn(4, 2, 64, device=DEV), torch.randn(4, 1, 64, device=DEV), torch.arange(4, device=DEV)
     f = ops.rotary_frequencies(64, device=DEV)
+    ops.rotary_embed(q, k, at, f)
+    for args, error in (((q, k, at[:3], f), ValueError), ((q, k, at.short(), f), TypeError), ((q, k[:3], at, f), ValueError),
+                        ((q, k.half(), at, f), TypeError), ((q[..., :32], k[..., :32], at, f), ValueError),
+                        ((q[0], None, at, f), ValueError), ((q, k[:, :0], at, f), ValueError), ((q.int(), None, at, f), TypeError),
+                        ((q, k, at, ops.rotary_frequencies(64, sections=(12, 10, 10), device=DEV)), ValueError)):
+        with pytest.raises(error, match="rotary_embed"):
+            ops.rotary_embed(*args)
     with pytest.raises(ValueError, match="one device"):
         ops.rotary_embed(q, None, torch.arange(4), f)
     with pytest.raises(ValueError, match="one device"):
@@ -240,6 +250,44 @@ def test_attention_results_do_not_depend_on_company():
         assert torch.equal(alone, out[q0:q0 + n])
 
 
+def test_attention_refusals():
+    q, k, v, qo, ko, kl, _ = _case([3, 2], [3, 4], 4, 2, 16, BF16)
+
+    def call(**change):
+        given = dict(query=q, key=k, value=v, q_offsets=qo, k_offsets=ko, k_lengths=kl, scale=None)
+        given.update(change)
+        return ops.packed_attention(**given)
+
+    call()
+    for change, error in ((dict(query=q[None]), ValueError), (dict(value=v[:-1]), ValueError),
+                          (dict(key=k[:, :0], value=v[:, :0]), ValueError), (dict(query=q[:, :3]), ValueError),
+                          (dict(key=k.half()), TypeError), (dict(q_offsets=qo.long()), TypeError),
+                          (dict(q_offsets=qo[::2]), TypeError), (dict(k_offsets=ko[:2]), ValueError),
+                          (dict(k_lengths=kl[:1]), ValueError), (dict(q_offsets=qo[:0], k_offsets=ko[:0]), ValueError),
+                          (dict(scale=0.0), ValueError), (dict(scale=math.nan), ValueError), (dict(scale=math.inf), ValueError),
+                          (dict(k_offsets=None, k_lengths=None), ValueError), (dict(key=k.cpu()), ValueError),
+                          (dict(k_offsets=ko.cpu()), ValueError)):
+        with pytest.raises(error, match="packed_attention"):
+            call(**change)
+
+
+def test_uncovered_calls_take_the_definitions():
+    """Types and head sizes without a kernel, and forward-mode tangents."""
+    import torch.autograd.forward_ad as fwad
+
+    q, k, v, qo, ko, kl, spans = _case([30, 2], [30, 7], 4, 2, 20, BF16, stale=0.0)
+    for dtype in (BF16, torch.float32, torch.float64):
+        x = [t.to(dtype) for t in (q, k, v)]
+        oracle.assert_close(ops.packed_attention(*x, qo, ko, k_lengths=kl), *oracle.attention(*x, spans, 20 ** -0.5)["out"])
+    q, k, v, qo, ko, kl, spans = _case([30], [30], 4, 2, 64, BF16)
+    f = ops.rotary_frequencies(64, device=DEV)
+    with fwad.dual_level():
+        dual = fwad.make_dual(q, torch.ones_like(q))
+        assert fwad.unpack_dual(ops.packed_attention(dual, k, v, qo)).tangent is not None
+        tangent = fwad.unpack_dual(ops.rotary_embed(dual, k, torch.arange(30, device=DEV), f)[0]).tangent
+    oracle.assert_close(tangent, *oracle.rotary(torch.ones_like(q), torch.arange(30, device=DEV), f.turns * 2 * math.pi))
+
+
 @pytest.mark.parametrize("rows", [1, 140])
 def test_attention_reports_bad_offsets(rows):
     """Offsets that leave the tensors are caught by the kernels' own checks: the sequence is skipped."""
@@ -325,3 +373,13 @@ def test_gradient_against_differences():
     want = oracle.attention(q, k, v, spans, 0.125, weight)
     allowed = sum((want[n][1] * s.abs()).sum() for n, s in zip(("dq", "dk", "dv"), steps))
     assert abs(slope - (value(1) - value(-1)) / (2 * h)) <= allowed + 1e-6 * abs(slope) + 1e-3
+
+
+def test_gradients_of_gradients_are_refused():
+    q, k, v, qo, *_ = _case([20], [20], 4, 2, 64, BF16)
+    f = ops.rotary_frequencies(64, device=DEV)
+    q.requires_grad_()
+    for out in (ops.packed_attention(q, k, v, qo), ops.rotary_embed(q, None, torch.arange(20, device=DEV), f)[0]):
+        (grad,) = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            grad.sum().backward()
