@@ -9,7 +9,10 @@
 //   warps 4-7  softmax of tile 1
 //   warp 8     TMA producer (K and V through rings of two stages); clears the V rows behind the last
 //              key, so that whatever lies there (another sequence, NaN) never meets a product
-//   warp 9     MMA issuer: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM
+//   warp 9     MMA issuer: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM (one elected thread in a
+//              branch of its own: a product then takes the pipe's 64 cycles, against 91 to 105 where
+//              the whole warp runs the loop and elects a lane for every instruction)
+//   warps 10-11 only complete the third warpgroup, which hands registers to the other two
 // While one tile is in its softmax the tensor core works for the other.  The running maximum is
 // only followed when it grows by more than 2^8: until then the scores are taken relative to the
 // old one, which leaves the quotient unchanged.  Sums, maxima and O are FP32; P is rounded to the
@@ -21,15 +24,21 @@
 #include "packed_common.cuh"
 #include "tensormap.h"
 
+#include <type_traits>
+
 namespace agb {
 namespace {
 
 constexpr int KV_STAGES = 2;
 constexpr int ROWS = 128;          // rows of a score tile, keys of a key tile
 constexpr int HALF_BYTES = 16384;  // 128 rows x 64 elements
-constexpr int FWD_THREADS = 320;
+constexpr int FWD_THREADS = 384;  // three warpgroups: softmax of tile 0, of tile 1, the rest
+constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;  // 2 x 208 + 80 fit the launch's 3 x 168
 constexpr uint32_t COL_S = 0, COL_O = 256;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
+// Of every eight pairs of unmasked scores, how many take the exponential of the FMA pipe: the
+// special-function unit alone (16 a cycle) is as slow as the products of a tile.
+constexpr int FMA_PAIRS = 2;
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int DP>
@@ -88,8 +97,8 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int unit = int(blockIdx.x / (unsigned(p.splits) * unsigned(p.head_units)));
 
   if (warp == 0) {
-    const PackedSpan span = find_unit(unit, step, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
-                                      p.total_q, p.total_k, head_unit == 0 && split == 0 ? p.status : nullptr);
+    const PackedSpan span = find_piece(unit, step, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
+                                       p.total_q, p.total_k, head_unit == 0 && split == 0 ? p.status : nullptr);
     if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
   }
   if (warp == 1 && lane == 0) {
@@ -123,8 +132,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
   const PackedSpan span = *reinterpret_cast<const PackedSpan*>(span_smem);
 
-  // The tiles of this CTA.  Long ones come first within a sequence: they decide how long the
-  // launch takes.
+  // The tiles of this CTA.
   int head[2], first[2], rows[2], tiles[2];  // first: row within the sequence
   int kv_head = 0, lo = 0, hi = 0;           // range of key tiles
   if (p.paired) {
@@ -136,9 +144,8 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   kv_head = head[0] / p.group;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int pieces = (span.rows + step - 1) / step;
-    first[t] = (pieces - 1 - span.unit_in_sequence) * step + (p.paired ? 0 : t * ROWS);
-    rows[t] = span.unit_in_sequence < 0 || span.rows == 0 ? 0 : max(0, min(ROWS, span.rows - first[t]));
+    first[t] = span.unit_in_sequence * step + (p.paired ? 0 : t * ROWS);
+    rows[t] = span.unit_in_sequence < 0 ? 0 : max(0, min(ROWS, span.rows - first[t]));
     const int seen = min(span.keys, span.keys - span.rows + first[t] + rows[t]);  // keys of the last row
     tiles[t] = rows[t] == 0 || seen <= 0 ? 0 : (seen + ROWS - 1) / ROWS;
   }
@@ -155,6 +162,8 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int last_valid = span.keys - (hi - 1) * ROWS;
   const bool ragged = n > 0 && last_valid < ROWS;
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp == 8) {
     // ------------------------------------------------------------------ TMA producer
     bool ok = true;
@@ -198,7 +207,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else if (warp == 9) {
     // -------------------------------------------------------------------- MMA issuer
-    if (n > 0) {  // the whole warp runs the loop; one elected lane issues
+    if (n > 0 && elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // both K-major over d
       constexpr uint32_t idesc_o = make_idesc_16(FP16, ROWS, DP, 0, 1);    // P from TMEM, V MN-major
       auto scores = [&](int t, int j) {
@@ -207,50 +216,53 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-          tc_mma_ss_w(tmem_base + COL_S + t * 128, make_smem_desc(q_addr + off, 16, 1024),
-                      make_smem_desc(k_addr + off, 16, 1024), idesc_s, kk != 0);
+          tc_mma_ss(tmem_base + COL_S + t * 128, make_smem_desc(q_addr + off, 16, 1024),
+                    make_smem_desc(k_addr + off, 16, 1024), idesc_s, kk != 0);
         }
-        tc_commit_w(&s_full[t]);
+        tc_commit(&s_full[t]);
       };
-      bool ok = mbar_wait_w(q_full, 0, guard, kTimeoutMma) && mbar_wait_w(&k_full[0], 0, guard, kTimeoutMma);
+      bool ok = mbar_wait(q_full, 0, guard, kTimeoutMma) && mbar_wait(&k_full[0], 0, guard, kTimeoutMma);
       if (ok) {
         tc_fence_after_sync();
         for (int t = 0; t < 2; ++t)
           if (tiles[t] > 0) scores(t, 0);
-        tc_commit_w(&k_empty[0]);
+        tc_commit(&k_empty[0]);
       }
       for (int j = 0; j < n && ok; ++j) {
         const int st = j % KV_STAGES;
         const bool more = j + 1 < n;
-        if (!mbar_wait_w(&v_full[st], (j / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
-        if (!more && ragged && !mbar_wait_w(v_clean, 0, guard, kTimeoutMma)) { ok = false; break; }
-        if (more && !mbar_wait_w(&k_full[(j + 1) % KV_STAGES], ((j + 1) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
+        if (!mbar_wait(&v_full[st], (j / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
+        if (!more && ragged && !mbar_wait(v_clean, 0, guard, kTimeoutMma)) { ok = false; break; }
+        if (more && !mbar_wait(&k_full[(j + 1) % KV_STAGES], ((j + 1) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
         const uint32_t v_addr = smem_u32(sV + st * TILE_BYTES);
         for (int t = 0; t < 2 && ok; ++t) {
           if (j >= tiles[t]) continue;
 #pragma unroll
           for (int c = 0; c < 2 && ok; ++c) {
-            if (!mbar_wait_w(&p_ready[2 * t + c], j & 1, guard, kTimeoutMma)) { ok = false; break; }
+            if (!mbar_wait(&p_ready[2 * t + c], j & 1, guard, kTimeoutMma)) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4) {
               const int kk = c * 4 + k4;  // 16 keys: P advances 8 packed columns, V 16 rows (2048 B)
-              tc_mma_ts_w(tmem_base + COL_O + t * 128, tmem_base + COL_S + t * 128 + kk * 8,
-                          make_smem_desc(v_addr + kk * 2048, HALF_BYTES, 1024), idesc_o, (j | kk) != 0);
+              tc_mma_ts(tmem_base + COL_O + t * 128, tmem_base + COL_S + t * 128 + kk * 8,
+                        make_smem_desc(v_addr + kk * 2048, HALF_BYTES, 1024), idesc_o, (j | kk) != 0);
             }
           }
           if (!ok) break;
           // behind the product above, which reads P from the buffer these scores refill: the
           // tensor core executes one thread's operations in issue order
           if (j + 1 < tiles[t]) scores(t, j + 1);
-          else tc_commit_w(&o_done[t]);
+          else tc_commit(&o_done[t]);
         }
         if (!ok) break;
-        tc_commit_w(&v_empty[st]);
-        if (more) tc_commit_w(&k_empty[(j + 1) % KV_STAGES]);
+        tc_commit(&v_empty[st]);
+        if (more) tc_commit(&k_empty[(j + 1) % KV_STAGES]);
       }
     }
+    __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     // ----------------------------------------------------------------------- softmax
     const int t = warp >> 2;
     const int quarter = warp & 3;                // TMEM lanes 32*quarter .. +31
@@ -276,7 +288,8 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(col_s + c * 32, s[c]);
       tmem_ld_wait();
-      if (seen_first < (j + 1) * ROWS) {  // the diagonal and the ragged last tile mask
+      const bool masked = seen_first < (j + 1) * ROWS;  // the diagonal and the ragged last tile
+      if (masked) {
         const int valid = seen - j * ROWS;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -318,23 +331,27 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
       const float2 shift2 = make_float2(-shift, -shift);
       float2 sum2 = make_float2(0.f, 0.f);
+      auto probabilities = [&](auto all) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t packed[32];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t packed[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint32_t* src = &s[2 * c + (i >> 4)][(2 * i) & 31];  // columns 2i, 2i+1 of half c
-          const float2 x = ffma2(make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), scale2, shift2);
-          const float2 e = make_float2(exp2f(x.x), exp2f(x.y));
-          sum2 = fadd2(sum2, e);
-          packed[i] = pack16<FP16>(e.x, e.y);
+          for (int i = 0; i < 32; ++i) {
+            const uint32_t* src = &s[2 * c + (i >> 4)][(2 * i) & 31];  // columns 2i, 2i+1 of half c
+            const float2 x = ffma2(make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), scale2, shift2);
+            const float2 e = decltype(all)::value && i % 8 < FMA_PAIRS ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
+            sum2 = fadd2(sum2, e);
+            packed[i] = pack16<FP16>(e.x, e.y);
+          }
+          tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
         }
-        tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
-      }
+      };
+      if (masked) probabilities(std::false_type{});
+      else probabilities(std::true_type{});
       l_sum += sum2.x + sum2.y;
     }
     // ---------------------------------------------------------------------- epilogue
@@ -364,7 +381,10 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
         if (row_ok) p.part_lse[at] = l_sum == 0.f ? -INFINITY : m_ref + log2f(l_sum);
       } else {
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * p.hq + my_head) * p.dim;
+        // Through the tile's own Q rows in shared memory (every product that read them is complete), so
+        // that a store writes whole rows: one row a thread would touch 32 lines an instruction.
+        uint8_t* stage = sQ + t * TILE_BYTES + quarter * 32 * DP * 2;
+        constexpr int WORDS = DP / 8;  // 16-byte words of a row, permuted against bank conflicts
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t o[32];
@@ -375,17 +395,25 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-          if (row_ok) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint4 v;
-              v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]) * inv, __uint_as_float(o[g * 8 + 1]) * inv);
-              v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]) * inv, __uint_as_float(o[g * 8 + 3]) * inv);
-              v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv);
-              v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv);
-              if (c * 32 + g * 8 < p.dim) *reinterpret_cast<uint4*>(dst + c * 32 + g * 8) = v;
-            }
+          for (int g = 0; g < 4; ++g) {
+            uint4 v;
+            v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]) * inv, __uint_as_float(o[g * 8 + 1]) * inv);
+            v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]) * inv, __uint_as_float(o[g * 8 + 3]) * inv);
+            v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv);
+            v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv);
+            *reinterpret_cast<uint4*>(stage + (lane * WORDS + ((c * 4 + g) ^ (lane & 7))) * 16) = v;
           }
+        }
+        __syncwarp();
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + ((row - lane) * p.hq + my_head) * p.dim;
+        const int words = p.dim / 8, live = my_rows - quarter * 32;
+#pragma unroll 4
+        for (int i = lane; i < 32 * WORDS; i += 32) {
+          const int r = i / WORDS, w = i % WORDS;
+          if (r < live && w < words)
+            *reinterpret_cast<uint4*>(dst + int64_t(r) * p.hq * p.dim + w * 8) =
+                *reinterpret_cast<const uint4*>(stage + (r * WORDS + (w ^ (r & 7))) * 16);
         }
         if (row_ok && p.lse)
           p.lse[int64_t(my_head) * p.total_q + row] =

@@ -77,6 +77,132 @@ __device__ inline PackedSpan find_unit(int unit, int step, bool by_keys, const i
   return span;
 }
 
+// The same for launches whose units differ in length: piece `rank` in the order of falling length, so
+// that no long piece starts last.  Per sequence the pieces' lengths follow from three numbers: `count`
+// pieces, the longest of `most`, each next one shorter by one, none counted longer than `cap`.  The
+// rank is found by a binary search over the length, each step one sum over the sequences, which two
+// registers a lane hold: up to MAX_RANKED sequences.  (With more there are enough pieces to even
+// out by themselves.)  Ranks behind the last piece own the rows that no sequence covers.
+constexpr int MAX_RANKED = 64;
+
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+
+__device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const int* __restrict__ q_offsets,
+                                         const int* __restrict__ k_offsets, const int* __restrict__ k_lengths,
+                                         int sequences, int64_t total_q, int64_t total_k, int* status) {
+  const int lane = threadIdx.x & 31;
+  int q0[2], q1[2], k0[2], k1[2], keys[2], count[2], most[2], cap[2];
+  bool bad = false;
+  const int end = (by_keys ? k_offsets : q_offsets)[sequences];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 32 * i;
+    const bool there = s < sequences;
+    const int at = there ? s : 0;
+    q0[i] = q_offsets[at];
+    q1[i] = q_offsets[at + (there ? 1 : 0)];
+    k0[i] = k_offsets[at];
+    k1[i] = k_offsets[at + (there ? 1 : 0)];
+    keys[i] = there && k_lengths ? k_lengths[at] : k1[i] - k0[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int rows = q1[i] - q0[i];
+    const bool fits = q0[i] >= 0 && rows >= 0 && q1[i] <= total_q && k0[i] >= 0 && k1[i] >= k0[i] &&
+                      k1[i] <= total_k && keys[i] >= 0 && keys[i] <= k1[i] - k0[i];
+    const bool there = lane + 32 * i < sequences;
+    bad = bad || !fits || (there && lane + i == 0 && (q0[0] != 0 || k0[0] != 0));
+    if (by_keys) {  // piece p is seen by the rows behind it: all of them while it lies before the first one
+      count[i] = there && fits ? (k1[i] - k0[i] + step - 1) / step : 0;
+      most[i] = ((keys[i] > rows ? keys[i] : rows) + step - 1) / step;
+      cap[i] = (rows + step - 1) / step;
+    } else {        // the last piece sees all keys, each earlier one a tile less
+      count[i] = there && fits ? (rows + step - 1) / step : 0;
+      most[i] = cap[i] = (keys[i] + step - 1) / step;
+    }
+  }
+  if (__any_sync(0xffffffffu, bad) && lane == 0 && status) atomicCAS(status, 0, kBadIndex);
+  PackedSpan span{-1, 0, 0, 0, 0, 0, 0};
+  const int all = warp_sum(count[0] + count[1]);
+  if (rank >= all) {
+    const int64_t total = by_keys ? total_k : total_q;
+    if (end < 0 || end > total) return span;
+    const int64_t first = end + int64_t(rank - all) * step;
+    span.unit_in_sequence = -2;
+    span.sequence = sequences;
+    span.q0 = span.k0 = int(first < total ? first : total);
+    span.rows = span.keys = span.room = int(first < total ? (total - first < step ? total - first : step) : 0);
+    return span;
+  }
+  // pieces of a lane's sequences that are at least `length` long
+  auto longer = [&](int i, int length) {
+    const int n = most[i] - length + 1;
+    return length > cap[i] || n < 0 ? 0 : (n < count[i] ? n : count[i]);
+  };
+  int low = 0x7fffffff, high = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (count[i] > 0) {
+      low = min(low, min(cap[i], most[i] - count[i] + 1));
+      high = max(high, cap[i]);
+    }
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high) + 1;  // nothing is this long
+  while (high - low > 1) {  // the greatest length that more than `rank` pieces reach
+    const int middle = low + (high - low) / 2;
+    if (warp_sum(longer(0, middle) + longer(1, middle)) > rank) low = middle;
+    else high = middle;
+  }
+  // the pieces of exactly this length, sequence by sequence
+  int behind[2], here[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    behind[i] = longer(i, low + 1);
+    here[i] = longer(i, low) - behind[i];
+  }
+  int index = rank - warp_sum(behind[0] + behind[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int before = here[i];  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += other;
+    }
+    const int sum = __shfl_sync(0xffffffffu, before, 31);
+    if (index < sum) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, index < before)) - 1;
+      const int nth = behind[i] + index - (before - here[i]);  // in the order of falling length
+      auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, owner); };
+      const int piece = by_keys ? nth : count[i] - 1 - nth;
+      span.unit_in_sequence = of(piece);
+      span.sequence = owner + 32 * i;
+      span.q0 = of(q0[i]);
+      span.rows = of(q1[i]) - span.q0;
+      span.k0 = of(k0[i]);
+      span.room = of(k1[i]) - span.k0;
+      span.keys = of(keys[i]);
+      return span;
+    }
+    index -= sum;
+  }
+  return span;
+}
+
+// Piece of a tile launch: ranked by length where that is possible.
+__device__ __forceinline__ PackedSpan find_piece(int unit, int step, bool by_keys, const int* __restrict__ q_offsets,
+                                                 const int* __restrict__ k_offsets, const int* __restrict__ k_lengths,
+                                                 int sequences, int64_t total_q, int64_t total_k, int* status) {
+  if (sequences <= MAX_RANKED)
+    return find_ranked(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
+  PackedSpan span = find_unit(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
+  if (!by_keys && span.unit_in_sequence >= 0) {  // late pieces of a sequence see the most keys and come first
+    const int pieces = (span.rows + step - 1) / step;
+    span.unit_in_sequence = pieces == 0 ? -1 : pieces - 1 - span.unit_in_sequence;
+  }
+  return span;
+}
+
 // Instruction descriptor for fp16 or bf16 operands (format 0 / 1), fp32 accumulation.
 __host__ __device__ constexpr uint32_t make_idesc_16(bool fp16, int m, int n, int a_mn_major, int b_mn_major) {
   return make_idesc_bf16(m, n, a_mn_major, b_mn_major) & (fp16 ? ~((1u << 7) | (1u << 10)) : ~0u);
@@ -94,6 +220,25 @@ template <bool FP16>
 __device__ __forceinline__ float2 unpack16(uint32_t v) {
   if (FP16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
   return make_float2(bf16_lo(v), bf16_hi(v));
+}
+
+// 2^x for two finite or NaN x, on the FMA pipe instead of the special-function unit: x = n + f with n the
+// nearest integer (Cody and Waite), a polynomial of degree 4 for 2^f that is off by at most 2.6e-6 of
+// it on [-1/2, 1/2] (fitted for the smallest largest relative error), and n added to the exponent.
+// x is taken as at least -126; NaN stays without a finite value of use.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x.x) : "f"(x.x));
+  asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(x.y) : "f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's last bits are n
+  const float2 t = fadd2(x, magic);
+  const float2 n = fadd2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = ffma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = ffma2(f, make_float2(0.00957010196f, 0.00957010196f), make_float2(0.0559178607f, 0.0559178607f));
+  p = ffma2(p, f, make_float2(0.240247448f, 0.240247448f));
+  p = ffma2(p, f, make_float2(0.693121815f, 0.693121815f));
+  p = ffma2(p, f, make_float2(0.999999261f, 0.999999261f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 }  // namespace agb
