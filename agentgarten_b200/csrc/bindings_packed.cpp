@@ -225,6 +225,7 @@ agb::PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, c
   a.scale = float(scale);
   a.status = status_word(q.device().index()).data_ptr<int>();
   a.splits = 1;
+  a.sm_count = sm_count(q);
   return a;
 }
 

@@ -57,6 +57,7 @@ struct PackedArgs {
   // [units, hkv, pieces, 16, dim] and [units, hkv, pieces, 16] with units = total_k / chunk + sequences
   // and pieces = packed_rows_pieces(hq / hkv) (unused when total_k <= chunk).
   int splits, chunk;
+  int sm_count;
   float* part_out;
   float* part_lse;
 };

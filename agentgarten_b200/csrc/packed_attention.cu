@@ -2,21 +2,29 @@
 //
 //   s = scale q k^T over the visible keys (j <= i + keys - rows), p = softmax(s), out = p v
 //
-// One CTA per (piece of a sequence's queries, two score tiles, key range).  The two tiles of 128
-// rows are two query heads that share a key head, or, when a key head has an odd number of query
-// heads, two neighbouring tiles of one head; both read the same K and V tiles.
-//   warps 0-3  softmax of tile 0: one query row per thread
+// Persistent CTAs, one an SM, work through items (piece of a sequence's queries, two score tiles, key
+// range) in the order of falling length, in a boustrophedon over the CTAs.  The two tiles of 128 rows
+// are two query heads that share a key head, or, when a key head has an odd number of query heads,
+// two neighbouring tiles of one head; both read the same K and V tiles.
+//   warps 0-3  softmax of tile 0: one query row per thread; then its output
 //   warps 4-7  softmax of tile 1
-//   warp 8     TMA producer (K and V through rings of two stages); clears the V rows behind the last
-//              key, so that whatever lies there (another sequence, NaN) never meets a product
+//   warp 8     TMA producer (K and V through rings of two stages, which run on from item to item)
 //   warp 9     MMA issuer: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM (one elected thread in a
 //              branch of its own: a product then takes the pipe's 64 cycles, against 91 to 105 where
 //              the whole warp runs the loop and elects a lane for every instruction)
-//   warps 10-11 only complete the third warpgroup, which hands registers to the other two
-// While one tile is in its softmax the tensor core works for the other.  The running maximum is
-// only followed when it grows by more than 2^8: until then the scores are taken relative to the
-// old one, which leaves the quotient unchanged.  Sums, maxima and O are FP32; P is rounded to the
-// tensors' type, as an operand of the tensor core has to be.
+//   warp 10    finds the items, one ahead
+//   warp 11    clears the V rows behind the last key, so that whatever lies there (another sequence,
+//              NaN) never meets a product
+// The third warpgroup hands registers to the other two.  While one tile is in its softmax the tensor
+// core works for the other, and while an item's outputs are written the next one's first scores are
+// computed; with a CTA for every item its start (finding the piece, first loads) and end cost 7 us,
+// as much as four key tiles.  The running maximum is only followed when it grows by more than 2^8:
+// until then the scores are taken relative to the old one, which leaves the quotient unchanged.
+// Sums, maxima and O are FP32; P is rounded to the tensors' type, as an operand of the tensor core has
+// to be.
+//
+// What bounds it: 2048 cycles of products for a pair of 128 x 128 tiles against about 1600 of one
+// tile's softmax, which has to lie between two of its products (2900 cycles measured).
 //
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512); P_t over the first half of S_t.
 #include "agb.h"
@@ -36,16 +44,14 @@ constexpr int FWD_THREADS = 384;  // three warpgroups: softmax of tile 0, of til
 constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;  // 2 x 208 + 80 fit the launch's 3 x 168
 constexpr uint32_t COL_S = 0, COL_O = 256;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
-// Of every eight pairs of unmasked scores, how many take the exponential of the FMA pipe: the
-// special-function unit alone (16 a cycle) is as slow as the products of a tile.
-constexpr int FMA_PAIRS = 2;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int STAGE_BYTES = 32 * 64;  // a warp's part of the output on its way: 32 rows x 64 bytes
 
 template <int DP>
 constexpr int fwd_smem() {
-  // Q_0, Q_1, K ring, V ring.  Never less than half of an SM's shared memory: two CTAs do not fit
-  // in its tensor memory, and the second would wait for the first in its allocation.
-  const int bytes = (2 + 2 * KV_STAGES) * (DP / 64) * HALF_BYTES + 1024 + 512;
+  // Q_0, Q_1, K ring, V ring, output stage.  Never less than half of an SM's shared memory: two CTAs do
+  // not fit in its tensor memory, and the second would wait for the first in its allocation.
+  const int bytes = (2 + 2 * KV_STAGES) * (DP / 64) * HALF_BYTES + 8 * STAGE_BYTES + 1024 + 1024;
   return bytes > 120 * 1024 ? bytes : 120 * 1024;
 }
 
@@ -57,11 +63,53 @@ struct FwdParams {
   float* lse;
   float* part_out; float* part_lse;
   int hq, dim, group, splits;
-  int head_units;   // CTAs side by side for one piece: hq / 2 (pairs of heads) or hq
+  int head_units;   // items side by side for one piece: hq / 2 (pairs of heads) or hq
   int paired;       // 1: the tiles are two heads, 0: two neighbouring row tiles
+  int64_t units;    // items, among them some without work
   float scale_log2;
   int* status;
 };
+
+// What the roles need of an item.  Per tile: head, first row within the sequence, rows, key tiles (from
+// the range's first on).
+enum : int { ITEM_END = 0, ITEM_TILES = 1, ITEM_UNCOVERED = 2 };
+struct Item {
+  int kind, split;
+  int head[2], first[2], rows[2], tiles[2];
+  int kv_head, q0, k0, query_rows, keys;
+  int lo, n;        // range of key tiles
+  int last_valid;   // keys that exist in the range's last tile (128 or more: all)
+};
+constexpr int ITEM_READERS = 11;  // eight softmax warps, producer, issuer, clearing warp
+
+__device__ inline Item make_item(const PackedSpan& span, const FwdParams& p, int head_unit, int split) {
+  Item item{};
+  const int step = p.paired ? ROWS : 2 * ROWS;
+  item.kind = span.unit_in_sequence == -2 ? ITEM_UNCOVERED : ITEM_TILES;
+  item.split = split;
+  item.q0 = span.q0;
+  item.k0 = span.k0;
+  item.query_rows = span.rows;
+  item.keys = span.keys;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    item.head[t] = p.paired ? 2 * head_unit + t : head_unit;
+    item.first[t] = span.unit_in_sequence * step + (p.paired ? 0 : t * ROWS);
+    item.rows[t] = item.kind == ITEM_TILES ? max(0, min(ROWS, span.rows - item.first[t])) : 0;
+    const int seen = min(span.keys, span.keys - span.rows + item.first[t] + item.rows[t]);  // keys of the last row
+    item.tiles[t] = item.rows[t] == 0 || seen <= 0 ? 0 : (seen + ROWS - 1) / ROWS;
+  }
+  item.kv_head = item.head[0] / p.group;
+  const int most = max(item.tiles[0], item.tiles[1]);
+  const int per = (most + p.splits - 1) / p.splits;
+  item.lo = min(most, split * per);
+  const int hi = min(most, item.lo + per);
+  item.n = hi - item.lo;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) item.tiles[t] = max(0, min(hi, item.tiles[t]) - item.lo);
+  item.last_valid = span.keys - (hi - 1) * ROWS;
+  return item;
+}
 
 template <int DP, bool FP16>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
@@ -74,36 +122,33 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   uint8_t* sQ = smem;
   uint8_t* sK = smem + 2 * TILE_BYTES;
   uint8_t* sV = sK + KV_STAGES * TILE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + KV_STAGES * TILE_BYTES);
+  uint8_t* sOut = sV + KV_STAGES * TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + 8 * STAGE_BYTES);
   uint64_t* q_full = bars;         // 1
-  uint64_t* k_full = bars + 1;     // [2]
-  uint64_t* k_empty = bars + 3;    // [2]
-  uint64_t* v_full = bars + 5;     // [2]
-  uint64_t* v_empty = bars + 7;    // [2]
-  uint64_t* s_full = bars + 9;     // [2 tiles] scores complete
-  uint64_t* p_ready = bars + 11;   // [2 tiles][2 halves of the keys] probabilities in TMEM (count 4)
-  uint64_t* o_done = bars + 15;    // [2 tiles] last product complete
-  uint64_t* v_clean = bars + 17;   // rows behind the last key cleared
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t* q_empty = bars + 1;    // last scores of an item complete
+  uint64_t* k_full = bars + 2;     // [2]
+  uint64_t* k_empty = bars + 4;    // [2]
+  uint64_t* v_full = bars + 6;     // [2]
+  uint64_t* v_empty = bars + 8;    // [2]
+  uint64_t* s_full = bars + 10;    // [2 tiles] scores complete
+  uint64_t* p_ready = bars + 12;   // [2 tiles][2 halves of the keys] probabilities in TMEM (count 4)
+  uint64_t* o_done = bars + 16;    // [2 tiles] last product complete
+  uint64_t* v_ragged = bars + 18;  // an item's ragged last V tile is there
+  uint64_t* v_clean = bars + 19;   // and its rows behind the last key are cleared
+  uint64_t* item_full = bars + 20; // [2]
+  uint64_t* item_empty = bars + 22;  // [2] (count ITEM_READERS)
+  Item* items = reinterpret_cast<Item*>(bars + 24);  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const WaitGuard guard{abort_flag, p.status};
-  const int step = p.paired ? ROWS : 2 * ROWS;
-  const int split = int(blockIdx.x % unsigned(p.splits));
-  const int head_unit = int((blockIdx.x / unsigned(p.splits)) % unsigned(p.head_units));
-  const int unit = int(blockIdx.x / (unsigned(p.splits) * unsigned(p.head_units)));
 
-  if (warp == 0) {
-    const PackedSpan span = find_piece(unit, step, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
-                                       p.total_q, p.total_k, head_unit == 0 && split == 0 ? p.status : nullptr);
-    if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
-  }
   if (warp == 1 && lane == 0) {
     *abort_flag = 0;
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -113,7 +158,10 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       mbar_init(&p_ready[2 * i], 4);
       mbar_init(&p_ready[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], ITEM_READERS);
     }
+    mbar_init(v_ragged, 1);
     mbar_init(v_clean, 1);
     mbar_fence_init();
   }
@@ -130,62 +178,48 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const PackedSpan span = *reinterpret_cast<const PackedSpan*>(span_smem);
 
-  // The tiles of this CTA.
-  int head[2], first[2], rows[2], tiles[2];  // first: row within the sequence
-  int kv_head = 0, lo = 0, hi = 0;           // range of key tiles
-  if (p.paired) {
-    head[0] = 2 * head_unit;
-    head[1] = head[0] + 1;
-  } else {
-    head[0] = head[1] = head_unit;
-  }
-  kv_head = head[0] / p.group;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    first[t] = span.unit_in_sequence * step + (p.paired ? 0 : t * ROWS);
-    rows[t] = span.unit_in_sequence < 0 ? 0 : max(0, min(ROWS, span.rows - first[t]));
-    const int seen = min(span.keys, span.keys - span.rows + first[t] + rows[t]);  // keys of the last row
-    tiles[t] = rows[t] == 0 || seen <= 0 ? 0 : (seen + ROWS - 1) / ROWS;
-  }
-  {
-    const int most = max(tiles[0], tiles[1]);
-    const int per = (most + p.splits - 1) / p.splits;
-    lo = min(most, split * per);
-    hi = min(most, lo + per);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) tiles[t] = max(0, min(hi, tiles[t]) - lo);
-  }
-  const int n = hi - lo;
-  // Keys of the last tile of the sequence that exist; its rows behind them are cleared.
-  const int last_valid = span.keys - (hi - 1) * ROWS;
-  const bool ragged = n > 0 && last_valid < ROWS;
+  // The i-th item in its slot of the ring; a reader frees the slot once it has what it needs.
+  auto item_wait = [&](int i, int code) { return mbar_wait(&item_full[i & 1], (i >> 1) & 1, guard, code); };
+  auto item_free = [&](int i) { mbar_arrive(&item_empty[i & 1]); };
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-  if (warp == 8) {
-    // ------------------------------------------------------------------ TMA producer
-    bool ok = true;
-    if (n > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == 8) {
+      // ------------------------------------------------------------------ TMA producer
       if (lane == 0) {
-        mbar_expect_tx(q_full, ((tiles[0] > 0) + (tiles[1] > 0)) * TILE_BYTES);
-        for (int t = 0; t < 2; ++t)
-          if (tiles[t] > 0)
+        bool ok = true;
+        int loads = 0;  // key tiles so far
+        for (int i = 0, used = 0; ok; ++i) {
+          if (!item_wait(i, kTimeoutProducer)) { ok = false; break; }
+          const Item& it = items[i & 1];
+          const int kind = it.kind, n = it.n, kv_head = it.kv_head, q0 = it.q0, row0 = it.k0 + it.lo * ROWS;
+          const int head[2] = {it.head[0], it.head[1]}, first[2] = {it.first[0], it.first[1]};
+          const bool there[2] = {it.tiles[0] > 0, it.tiles[1] > 0};
+          item_free(i);
+          if (kind == ITEM_END) break;
+          if (n == 0) continue;
+          if (!mbar_wait(q_empty, (used & 1) ^ 1, guard, kTimeoutProducer)) { ok = false; break; }
+          ++used;
+          mbar_expect_tx(q_full, (there[0] + there[1]) * TILE_BYTES);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (there[t])
+              for (int a = 0; a < ATOMS; ++a)
+                tma_load_3d(sQ + t * TILE_BYTES + a * HALF_BYTES, &tm_q, q_full, a * 64, head[t], q0 + first[t]);
+          for (int j = 0; j < n && ok; ++j, ++loads) {
+            const int st = loads % KV_STAGES;
+            const uint32_t ph = ((loads / KV_STAGES) & 1) ^ 1;
+            const int row = row0 + j * ROWS;
+            if (!mbar_wait(&k_empty[st], ph, guard, kTimeoutProducer)) { ok = false; break; }
+            mbar_expect_tx(&k_full[st], TILE_BYTES);
             for (int a = 0; a < ATOMS; ++a)
-              tma_load_3d(sQ + t * TILE_BYTES + a * HALF_BYTES, &tm_q, q_full, a * 64, head[t], span.q0 + first[t]);
-        for (int j = 0; j < n && ok; ++j) {
-          const int st = j % KV_STAGES;
-          const uint32_t ph = ((j / KV_STAGES) & 1) ^ 1;
-          const int row = span.k0 + (lo + j) * ROWS;
-          if (!mbar_wait(&k_empty[st], ph, guard, kTimeoutProducer)) { ok = false; break; }
-          mbar_expect_tx(&k_full[st], TILE_BYTES);
-          for (int a = 0; a < ATOMS; ++a)
-            tma_load_3d(sK + st * TILE_BYTES + a * HALF_BYTES, &tm_k, &k_full[st], a * 64, kv_head, row);
-          if (!mbar_wait(&v_empty[st], ph, guard, kTimeoutProducer)) { ok = false; break; }
-          mbar_expect_tx(&v_full[st], TILE_BYTES);
-          for (int a = 0; a < ATOMS; ++a)
-            tma_load_3d(sV + st * TILE_BYTES + a * HALF_BYTES, &tm_v, &v_full[st], a * 64, kv_head, row);
+              tma_load_3d(sK + st * TILE_BYTES + a * HALF_BYTES, &tm_k, &k_full[st], a * 64, kv_head, row);
+            if (!mbar_wait(&v_empty[st], ph, guard, kTimeoutProducer)) { ok = false; break; }
+            mbar_expect_tx(&v_full[st], TILE_BYTES);
+            for (int a = 0; a < ATOMS; ++a)
+              tma_load_3d(sV + st * TILE_BYTES + a * HALF_BYTES, &tm_v, &v_full[st], a * 64, kv_head, row);
+          }
         }
         if (!ok || *abort_flag) {
           // give in-flight copies time to land before shared memory is released
@@ -193,74 +227,135 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           while (global_timer_ns() - start < 100000ull) {}
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (ragged && ok && mbar_wait_w(&v_full[(n - 1) % KV_STAGES], ((n - 1) / KV_STAGES) & 1, guard, kTimeoutProducer)) {
+    } else if (warp == 9) {
+      // -------------------------------------------------------------------- MMA issuer
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // both K-major over d
+        constexpr uint32_t idesc_o = make_idesc_16(FP16, ROWS, DP, 0, 1);    // P from TMEM, V MN-major
+        auto scores = [&](int t, int st) {
+          const uint32_t q_addr = smem_u32(sQ + t * TILE_BYTES);
+          const uint32_t k_addr = smem_u32(sK + st * TILE_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+            tc_mma_ss(tmem_base + COL_S + t * 128, make_smem_desc(q_addr + off, 16, 1024),
+                      make_smem_desc(k_addr + off, 16, 1024), idesc_s, kk != 0);
+          }
+          tc_commit(&s_full[t]);
+        };
+        bool ok = true;
+        int loads = 0;             // key tiles of earlier items
+        uint32_t done[2] = {0, 0}; // tiles' score blocks of earlier items
+        for (int i = 0, used = 0, cleaned = 0; ok; ++i) {
+          if (!item_wait(i, kTimeoutMma)) break;
+          const Item& it = items[i & 1];
+          const int kind = it.kind, n = it.n;
+          const int tiles[2] = {it.tiles[0], it.tiles[1]};
+          const bool ragged = it.last_valid < ROWS;
+          item_free(i);
+          if (kind == ITEM_END) break;
+          if (n == 0) continue;
+          ok = mbar_wait(q_full, used & 1, guard, kTimeoutMma) &&
+               mbar_wait(&k_full[loads % KV_STAGES], (loads / KV_STAGES) & 1, guard, kTimeoutMma);
+          if (!ok) break;
+          ++used;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (tiles[t] > 0) scores(t, loads % KV_STAGES);
+          tc_commit(&k_empty[loads % KV_STAGES]);
+          if (n == 1) tc_commit(q_empty);
+          for (int j = 0; j < n && ok; ++j) {
+            const int st = (loads + j) % KV_STAGES, next = (loads + j + 1) % KV_STAGES;
+            const bool more = j + 1 < n;
+            if (!mbar_wait(&v_full[st], ((loads + j) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
+            if (!more && ragged) {
+              mbar_arrive(v_ragged);
+              if (!mbar_wait(v_clean, cleaned++ & 1, guard, kTimeoutMma)) { ok = false; break; }
+            }
+            if (more && !mbar_wait(&k_full[next], ((loads + j + 1) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
+            const uint32_t v_addr = smem_u32(sV + st * TILE_BYTES);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || j >= tiles[t]) continue;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (!ok || !mbar_wait(&p_ready[2 * t + c], (done[t] + j) & 1, guard, kTimeoutMma)) { ok = false; break; }
+                tc_fence_after_sync();
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4) {
+                  const int kk = c * 4 + k4;  // 16 keys: P advances 8 packed columns, V 16 rows (2048 B)
+                  tc_mma_ts(tmem_base + COL_O + t * 128, tmem_base + COL_S + t * 128 + kk * 8,
+                            make_smem_desc(v_addr + kk * 2048, HALF_BYTES, 1024), idesc_o, (j | kk) != 0);
+                }
+              }
+              if (!ok) break;
+              // behind the product above, which reads P from the buffer these scores refill: the
+              // tensor core executes one thread's operations in issue order
+              if (j + 1 < tiles[t]) scores(t, next);
+              else tc_commit(&o_done[t]);
+            }
+            if (!ok) break;
+            tc_commit(&v_empty[st]);
+            if (more) tc_commit(&k_empty[next]);
+            if (j + 2 == n) tc_commit(q_empty);
+          }
+          loads += n;
+          done[0] += tiles[0];
+          done[1] += tiles[1];
+        }
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // ------------------------------------------------------------------------ items
+      const int64_t ctas = gridDim.x;
+      int i = 0;
+      for (int64_t round = 0;; ++round) {
+        const int64_t unit = round * ctas + (round & 1 ? ctas - 1 - blockIdx.x : blockIdx.x);
+        const bool last = round * ctas >= p.units;
+        if (!last && unit >= p.units) continue;
+        Item item{};
+        if (!last) {
+          const int split = int(unit % p.splits);
+          const int head_unit = int(unit / p.splits % p.head_units);
+          const PackedSpan span = find_piece(int(unit / p.splits / p.head_units), p.paired ? ROWS : 2 * ROWS, false,
+                                             p.q_offsets, p.k_offsets, p.k_lengths, p.sequences, p.total_q, p.total_k,
+                                             head_unit == 0 && split == 0 ? p.status : nullptr);
+          if (span.unit_in_sequence == -1 || (span.unit_in_sequence == -2 && span.rows == 0)) continue;
+          item = make_item(span, p, head_unit, split);
+        }
+        if (!mbar_wait_w(&item_empty[i & 1], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer)) break;
+        if (lane == 0) {
+          items[i & 1] = item;
+          mbar_arrive(&item_full[i & 1]);
+        }
+        __syncwarp();
+        if (last) break;
+        ++i;
+      }
+    } else {
+      // ------------------------------------------------------------- rows behind the keys
+      int loads = 0;
+      for (int i = 0, cleaned = 0;; ++i) {
+        if (!mbar_wait_w(&item_full[i & 1], (i >> 1) & 1, guard, kTimeoutProducer)) break;
+        const int kind = items[i & 1].kind, n = items[i & 1].n, valid = items[i & 1].last_valid;
+        __syncwarp();
+        if (lane == 0) item_free(i);
+        if (kind == ITEM_END) break;
+        if (n == 0) continue;
+        loads += n;
+        if (valid >= ROWS) continue;
+        if (!mbar_wait_w(v_ragged, cleaned++ & 1, guard, kTimeoutProducer)) break;
         // a row is 128 bytes of each atom whatever the swizzle, which permutes within the row
-        uint8_t* tile = sV + ((n - 1) % KV_STAGES) * TILE_BYTES;
-        for (int i = last_valid * 8 + lane; i < ROWS * 8; i += 32)
+        uint8_t* tile = sV + ((loads - 1) % KV_STAGES) * TILE_BYTES;
+        for (int w = valid * 8 + lane; w < ROWS * 8; w += 32)
           for (int a = 0; a < ATOMS; ++a)
-            *reinterpret_cast<uint4*>(tile + a * HALF_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(tile + a * HALF_BYTES + w * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_clean);
       }
     }
-  } else if (warp == 9) {
-    // -------------------------------------------------------------------- MMA issuer
-    if (n > 0 && elect_one()) {
-      constexpr uint32_t idesc_s = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // both K-major over d
-      constexpr uint32_t idesc_o = make_idesc_16(FP16, ROWS, DP, 0, 1);    // P from TMEM, V MN-major
-      auto scores = [&](int t, int j) {
-        const uint32_t q_addr = smem_u32(sQ + t * TILE_BYTES);
-        const uint32_t k_addr = smem_u32(sK + (j % KV_STAGES) * TILE_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-          tc_mma_ss(tmem_base + COL_S + t * 128, make_smem_desc(q_addr + off, 16, 1024),
-                    make_smem_desc(k_addr + off, 16, 1024), idesc_s, kk != 0);
-        }
-        tc_commit(&s_full[t]);
-      };
-      bool ok = mbar_wait(q_full, 0, guard, kTimeoutMma) && mbar_wait(&k_full[0], 0, guard, kTimeoutMma);
-      if (ok) {
-        tc_fence_after_sync();
-        for (int t = 0; t < 2; ++t)
-          if (tiles[t] > 0) scores(t, 0);
-        tc_commit(&k_empty[0]);
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        const int st = j % KV_STAGES;
-        const bool more = j + 1 < n;
-        if (!mbar_wait(&v_full[st], (j / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
-        if (!more && ragged && !mbar_wait(v_clean, 0, guard, kTimeoutMma)) { ok = false; break; }
-        if (more && !mbar_wait(&k_full[(j + 1) % KV_STAGES], ((j + 1) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
-        const uint32_t v_addr = smem_u32(sV + st * TILE_BYTES);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= tiles[t]) continue;
-#pragma unroll
-          for (int c = 0; c < 2 && ok; ++c) {
-            if (!mbar_wait(&p_ready[2 * t + c], j & 1, guard, kTimeoutMma)) { ok = false; break; }
-            tc_fence_after_sync();
-#pragma unroll
-            for (int k4 = 0; k4 < 4; ++k4) {
-              const int kk = c * 4 + k4;  // 16 keys: P advances 8 packed columns, V 16 rows (2048 B)
-              tc_mma_ts(tmem_base + COL_O + t * 128, tmem_base + COL_S + t * 128 + kk * 8,
-                        make_smem_desc(v_addr + kk * 2048, HALF_BYTES, 1024), idesc_o, (j | kk) != 0);
-            }
-          }
-          if (!ok) break;
-          // behind the product above, which reads P from the buffer these scores refill: the
-          // tensor core executes one thread's operations in issue order
-          if (j + 1 < tiles[t]) scores(t, j + 1);
-          else tc_commit(&o_done[t]);
-        }
-        if (!ok) break;
-        tc_commit(&v_empty[st]);
-        if (more) tc_commit(&k_empty[(j + 1) % KV_STAGES]);
-      }
-    }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     // ----------------------------------------------------------------------- softmax
@@ -270,164 +365,180 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int my_row = quarter * 32 + lane;
     const uint32_t col_s = tmem_base + lane_base + COL_S + t * 128;
     const uint32_t col_o = tmem_base + lane_base + COL_O + t * 128;
-    const int my_tiles = t == 0 ? tiles[0] : tiles[1];
-    const int my_first = t == 0 ? first[0] : first[1];
-    const int my_rows = t == 0 ? rows[0] : rows[1];
-    const int my_head = t == 0 ? head[0] : head[1];
-    // keys that this row and the tile's first row see, from the first key of the range on
-    const int before = span.keys - span.rows + my_first + 1 - lo * ROWS;
-    const int seen = min(span.keys - lo * ROWS, before + my_row);
-    const int seen_first = min(span.keys - lo * ROWS, before);
-    float m_ref = -INFINITY;                     // reference maximum (log2 domain)
-    float l_sum = 0.f;
+    uint8_t* stage = sOut + warp * STAGE_BYTES;
     bool ok = true;
-    for (int j = 0; j < my_tiles && ok; ++j) {
-      if (!mbar_wait(&s_full[t], j & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
-      tc_fence_after_sync();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(col_s + c * 32, s[c]);
-      tmem_ld_wait();
-      const bool masked = seen_first < (j + 1) * ROWS;  // the diagonal and the ragged last tile
-      if (masked) {
-        const int valid = seen - j * ROWS;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i >= valid) s[c][i] = 0xff800000u;  // -inf
+    uint32_t done = 0, outs = 0;                 // score blocks and outputs of earlier items
+    for (int i = 0; ok; ++i) {
+      if (!item_wait(i, kTimeoutSoftmax)) break;
+      const Item& it = items[i & 1];
+      const int kind = it.kind, my_tiles = it.tiles[t], my_rows = it.rows[t], my_head = it.head[t], split = it.split;
+      const int q_row = it.q0 + it.first[t];     // first row of the tile
+      // keys that this row and the tile's first row see, from the first key of the range on
+      const int before = it.keys - it.query_rows + it.first[t] + 1 - it.lo * ROWS;
+      const int seen = min(it.keys - it.lo * ROWS, before + my_row);
+      const int seen_first = min(it.keys - it.lo * ROWS, before);
+      const int uncovered0 = it.q0, uncovered = it.query_rows;
+      __syncwarp();
+      if (lane == 0) item_free(i);
+      if (kind == ITEM_END) break;
+      if (kind == ITEM_UNCOVERED) {  // zeros (the join writes them for split launches)
+        const int words = p.dim / 8;
+        if (p.splits == 1 && (p.paired || t == 0))
+          for (int w = my_row; w < uncovered * words; w += ROWS) {
+            uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                            ((int64_t(uncovered0) + w / words) * p.hq + my_head) * p.dim + (w % words) * 8;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+          }
+        continue;
       }
-      float m4[4];
+      float m_ref = -INFINITY;                   // reference maximum (log2 domain)
+      float l_sum = 0.f;
+      for (int j = 0; j < my_tiles && ok; ++j) {
+        if (!mbar_wait(&s_full[t], (done + j) & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+        tc_fence_after_sync();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        m4[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(col_s + c * 32, s[c]);
+        tmem_ld_wait();
+        const bool masked = seen_first < (j + 1) * ROWS;  // the diagonal and the ragged last tile
+        if (masked) {
+          const int valid = seen - j * ROWS;
 #pragma unroll
-        for (int i = 2; i < 32; i += 2)
-          m4[c] = fmax3(m4[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-      }
-      const float m_tile = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * p.scale_log2;
-      // The previous product of this tile is complete: these scores were executed after it.
-      const bool grow = m_tile > m_ref + RESCALE_THRESHOLD;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = fmaxf(m_ref, m_tile);
-        const float alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);
-        if (j > 0) {
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= valid) s[c][k] = 0xff800000u;  // -inf
+        }
+        float m4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          m4[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+#pragma unroll
+          for (int k = 2; k < 32; k += 2) m4[c] = fmax3(m4[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+        }
+        const float m_tile = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * p.scale_log2;
+        // The previous product of this tile is complete: these scores were executed after it.
+        const bool grow = m_tile > m_ref + RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = fmaxf(m_ref, m_tile);
+          const float alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);
+          if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(col_o + c * 32, o);
-            tmem_ld_wait();
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(col_o + c * 32, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32(col_o + c * 32, o);
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st_32x32(col_o + c * 32, o);
+            }
+            tmem_st_wait();
           }
-          tmem_st_wait();
+          l_sum *= alpha;
+          m_ref = m_new;
         }
-        l_sum *= alpha;
-        m_ref = m_new;
+        // A row that has seen nothing yet keeps m_ref = -inf: its scores are -inf and the shift is 0.
+        const float shift = m_ref == -INFINITY ? 0.f : m_ref;
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        const float2 shift2 = make_float2(-shift, -shift);
+        float2 sums[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[k] = make_float2(0.f, 0.f);
+        // One pair of unmasked scores in four takes the exponential of the FMA pipe: a tile's share of
+        // the special-function unit (16 a cycle) is as long as its products.  1661 us against 1690
+        // without, 1708 for one in eight and 1747 for three in eight, at 16384 tokens.
+        auto probabilities = [&](auto all) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t packed[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const uint32_t* src = &s[2 * c + (k >> 4)][(2 * k) & 31];  // columns 2k, 2k+1 of half c
+              const float2 x = ffma2(make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), scale2, shift2);
+              const float2 e = decltype(all)::value && k % 4 == 3 ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
+              sums[k & 3] = fadd2(sums[k & 3], e);
+              packed[k] = pack16<FP16>(e.x, e.y);
+            }
+            tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
+          }
+        };
+        if (masked) probabilities(std::false_type{});
+        else probabilities(std::true_type{});
+        const float2 sum2 = fadd2(fadd2(sums[0], sums[1]), fadd2(sums[2], sums[3]));
+        l_sum += sum2.x + sum2.y;
       }
-      // A row that has seen nothing yet keeps m_ref = -inf: its scores are -inf and the shift is 0.
-      const float shift = m_ref == -INFINITY ? 0.f : m_ref;
-      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-      const float2 shift2 = make_float2(-shift, -shift);
-      float2 sum2 = make_float2(0.f, 0.f);
-      auto probabilities = [&](auto all) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t packed[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint32_t* src = &s[2 * c + (i >> 4)][(2 * i) & 31];  // columns 2i, 2i+1 of half c
-            const float2 x = ffma2(make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), scale2, shift2);
-            const float2 e = decltype(all)::value && i % 8 < FMA_PAIRS ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
-            sum2 = fadd2(sum2, e);
-            packed[i] = pack16<FP16>(e.x, e.y);
-          }
-          tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
-          tmem_st_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
-        }
-      };
-      if (masked) probabilities(std::false_type{});
-      else probabilities(std::true_type{});
-      l_sum += sum2.x + sum2.y;
-    }
-    // ---------------------------------------------------------------------- epilogue
-    if (ok && my_tiles > 0) ok = mbar_wait(&o_done[t], 0, guard, kTimeoutEpilogue);
-    if (ok) {
+      done += my_tiles;
+      // ---------------------------------------------------------------------- output
+      if (ok && my_tiles > 0) ok = mbar_wait(&o_done[t], outs++ & 1, guard, kTimeoutEpilogue);
+      if (!ok) break;
       tc_fence_after_sync();
       const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
-      const bool row_ok = my_row < my_rows;
-      const int64_t row = int64_t(span.q0) + my_first + my_row;
-      if (p.splits > 1) {
-        const int64_t at = (int64_t(split) * p.total_q + row) * p.hq + my_head;
-        if (my_tiles > 0) {
-#pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(col_o + c * 32, o);
-            tmem_ld_wait();
-            if (row_ok) {
+      const bool partial = p.splits > 1;
+      const int live = min(32, my_rows - quarter * 32);   // rows of this warp
+      const int64_t row = int64_t(q_row) + quarter * 32;  // its first
+      const int64_t at = (partial ? int64_t(split) * p.total_q : 0) * p.hq + row * p.hq + my_head;
+      if (live > 0 && !(partial && my_tiles == 0)) {
+        // 64 bytes of every row at a time through shared memory, words permuted against bank conflicts:
+        // one row a thread would make a store touch 32 lines
+        uint8_t* put = stage + lane * 64;
+        const int flip = (lane >> 1) & 3;
+        auto flush = [&](uint8_t* dst, int64_t pitch, int bytes) {  // `bytes` left of a row from this chunk on
+          __syncwarp();
 #pragma unroll
-              for (int g = 0; g < 8; ++g)
-                if (c * 32 + g * 4 < p.dim)
-                  *reinterpret_cast<float4*>(p.part_out + at * p.dim + c * 32 + g * 4) =
-                      make_float4(__uint_as_float(o[g * 4]) * inv, __uint_as_float(o[g * 4 + 1]) * inv,
-                                  __uint_as_float(o[g * 4 + 2]) * inv, __uint_as_float(o[g * 4 + 3]) * inv);
-            }
+          for (int k = 0; k < 4; ++k) {
+            const int r = k * 8 + (lane >> 2), w = lane & 3;
+            if (r < live && w * 16 < bytes)
+              *reinterpret_cast<uint4*>(dst + r * pitch + w * 16) =
+                  *reinterpret_cast<const uint4*>(stage + r * 64 + (w ^ ((r >> 1) & 3)) * 16);
           }
-        }
-        if (row_ok) p.part_lse[at] = l_sum == 0.f ? -INFINITY : m_ref + log2f(l_sum);
-      } else {
-        // Through the tile's own Q rows in shared memory (every product that read them is complete), so
-        // that a store writes whole rows: one row a thread would touch 32 lines an instruction.
-        uint8_t* stage = sQ + t * TILE_BYTES + quarter * 32 * DP * 2;
-        constexpr int WORDS = DP / 8;  // 16-byte words of a row, permuted against bank conflicts
+          __syncwarp();
+        };
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
+          if (c * 32 >= p.dim) break;
           uint32_t o[32];
           if (my_tiles > 0) {
             tmem_ld_32x32(col_o + c * 32, o);
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0;
+            for (int k = 0; k < 32; ++k) o[k] = 0;
           }
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 v;
-            v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]) * inv, __uint_as_float(o[g * 8 + 1]) * inv);
-            v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]) * inv, __uint_as_float(o[g * 8 + 3]) * inv);
-            v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv);
-            v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv);
-            *reinterpret_cast<uint4*>(stage + (lane * WORDS + ((c * 4 + g) ^ (lane & 7))) * 16) = v;
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+          if (partial) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint4*>(put + (g ^ flip) * 16) =
+                    make_uint4(o[h * 16 + g * 4], o[h * 16 + g * 4 + 1], o[h * 16 + g * 4 + 2], o[h * 16 + g * 4 + 3]);
+              flush(reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 32 + h * 16), int64_t(p.hq) * p.dim * 4,
+                    (p.dim - c * 32 - h * 16) * 4);
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint4 v;
+              v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]), __uint_as_float(o[g * 8 + 1]));
+              v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]), __uint_as_float(o[g * 8 + 3]));
+              v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]), __uint_as_float(o[g * 8 + 5]));
+              v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]), __uint_as_float(o[g * 8 + 7]));
+              *reinterpret_cast<uint4*>(put + (g ^ flip) * 16) = v;
+            }
+            flush(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 32), int64_t(p.hq) * p.dim * 2,
+                  (p.dim - c * 32) * 2);
           }
         }
-        __syncwarp();
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + ((row - lane) * p.hq + my_head) * p.dim;
-        const int words = p.dim / 8, live = my_rows - quarter * 32;
-#pragma unroll 4
-        for (int i = lane; i < 32 * WORDS; i += 32) {
-          const int r = i / WORDS, w = i % WORDS;
-          if (r < live && w < words)
-            *reinterpret_cast<uint4*>(dst + int64_t(r) * p.hq * p.dim + w * 8) =
-                *reinterpret_cast<const uint4*>(stage + (r * WORDS + (w ^ (r & 7))) * 16);
-        }
-        if (row_ok && p.lse)
-          p.lse[int64_t(my_head) * p.total_q + row] =
-              l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
       }
-    }
-    // Rows behind the last sequence: zero (the merge does it for split launches).
-    if (span.unit_in_sequence == -2 && p.splits == 1) {
-      const int heads = p.paired ? 2 : 1;
-      const int words = heads * p.dim / 8;  // 16-byte words of this CTA's heads in a row
-      for (int i = int(threadIdx.x); i < span.rows * words; i += 256) {
-        uint16_t* dst = static_cast<uint16_t*>(p.out) +
-                        ((int64_t(span.q0) + i / words) * p.hq + head[0]) * p.dim + (i % words) * 8;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+      if (lane < live) {
+        const float log_sum = l_sum == 0.f ? -INFINITY : m_ref + log2f(l_sum);
+        if (partial) p.part_lse[at + int64_t(lane) * p.hq] = log_sum;
+        else if (p.lse) p.lse[int64_t(my_head) * p.total_q + row + lane] = log_sum * 0.6931471805599453f;
       }
     }
   }
@@ -451,21 +562,24 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const float* __restric
   if (unit >= total_q * hq) return;
   const int lane = threadIdx.x & 31;
   const int64_t row = unit / hq;
-  const int head = int(unit % hq);
+  const int head = int(unit - row * hq);
+  const bool covered = row < q_offsets[sequences];
+  after_previous_launch();
+  const int64_t stride = total_q * hq;
+  const float mine = covered && lane < splits ? part_lse[lane * stride + unit] : -INFINITY;  // splits <= 32
+  float top = mine;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float share = mine == -INFINITY ? 0.f : exp2f(mine - top);  // 0: that range held no visible key
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, weight = 0.f;
-  if (row < q_offsets[sequences]) {
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_lse[(s * total_q + row) * hq + head]);
-    for (int s = 0; s < splits; ++s) {
-      const int64_t at = (s * total_q + row) * hq + head;
-      const float l = part_lse[at];
-      if (l == -INFINITY) continue;  // that range held no visible key
-      const float w = exp2f(l - top);
-      weight += w;
-      if (lane * 4 < dim) {
-        const float4 o = *reinterpret_cast<const float4*>(part_out + at * dim + lane * 4);
-        sum.x += w * o.x; sum.y += w * o.y; sum.z += w * o.z; sum.w += w * o.w;
-      }
+  float weight = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float w = __shfl_sync(0xffffffffu, share, s);
+    weight += w;
+    if (w != 0.f && lane * 4 < dim) {
+      const float4 o = *reinterpret_cast<const float4*>(part_out + (s * stride + unit) * dim + lane * 4);
+      sum.x += w * o.x; sum.y += w * o.y; sum.z += w * o.z; sum.w += w * o.w;
     }
   }
   const float inv = weight == 0.f ? 0.f : 1.f / weight;
@@ -473,7 +587,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const float* __restric
     uint2 v;
     v.x = pack16<FP16>(sum.x * inv, sum.y * inv);
     v.y = pack16<FP16>(sum.z * inv, sum.w * inv);
-    *reinterpret_cast<uint2*>(out + (row * hq + head) * dim + lane * 4) = v;
+    *reinterpret_cast<uint2*>(out + unit * dim + lane * 4) = v;
   }
   if (lse && lane == 0)
     lse[head * total_q + row] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.6931471805599453f;
@@ -496,19 +610,18 @@ cudaError_t launch_tiles(const PackedArgs& a, const CUtensorMap& tq, const CUten
   p.scale_log2 = a.scale * LOG2E;
   p.status = a.status;
   const int step = p.paired ? ROWS : 2 * ROWS;
-  const int64_t grid = (a.total_q / step + a.sequences + 1) * p.head_units * p.splits;
-  if (grid > 2147483647ll) {
-    set_error_detail("packed_attention: too many tiles for one launch");
+  p.units = (a.total_q / step + a.sequences + 1) * p.head_units * p.splits;
+  const int64_t blocks = (a.total_q * a.hq + 7) / 8;
+  if (blocks > 2147483647ll) {
+    set_error_detail("packed_attention: too many rows for one launch");
     return cudaErrorInvalidValue;
   }
-  packed_tiles_kernel<DP, FP16><<<unsigned(grid), FWD_THREADS, fwd_smem<DP>(), stream>>>(tq, tk, tv, p);
-  if (a.splits > 1) {
-    const int64_t blocks = (a.total_q * a.hq + 7) / 8;
-    packed_join_kernel<FP16><<<unsigned(blocks), 256, 0, stream>>>(
-        a.part_out, a.part_lse, static_cast<uint16_t*>(a.out), a.lse, a.q_offsets, a.sequences, a.total_q, a.hq,
-        a.dim, a.splits);
-  }
-  return cudaGetLastError();
+  const unsigned grid = unsigned(p.units < a.sm_count ? p.units : a.sm_count);
+  packed_tiles_kernel<DP, FP16><<<grid, FWD_THREADS, fwd_smem<DP>(), stream>>>(tq, tk, tv, p);
+  const cudaError_t launched = cudaGetLastError();
+  if (launched != cudaSuccess || a.splits == 1) return launched;
+  return launch_behind(packed_join_kernel<FP16>, dim3(unsigned(blocks)), 256, 0, stream, a.part_out, a.part_lse,
+                       static_cast<uint16_t*>(a.out), a.lse, a.q_offsets, a.sequences, a.total_q, a.hq, a.dim, a.splits);
 }
 
 }  // namespace

@@ -283,21 +283,26 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
   }
 }
 
-// Joins the chunks of every row that had several: out = sum_c w_c o_c in chunk order.  One warp per
-// (query row, head).
+// Joins the chunks of every row that had several: out = sum_c w_c o_c.  One CTA per (query row, head);
+// its warps take chunks in turn and are added in warp order.
+constexpr int JOIN_WARPS = 8;
 template <bool FP16>
-__global__ void __launch_bounds__(256) packed_rows_join_kernel(const RowsParams p) {
-  const int64_t job = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (job >= p.total_q * p.hq) return;
-  const int lane = threadIdx.x & 31;
-  const int row = int(job / p.hq), head = int(job % p.hq);
+__global__ void __launch_bounds__(JOIN_WARPS * 32) packed_rows_join_kernel(const RowsParams p) {
+  __shared__ float4 partial[JOIN_WARPS][32];
+  __shared__ float weight[JOIN_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int row = int(blockIdx.x / unsigned(p.hq)), head = int(blockIdx.x % unsigned(p.hq));
   // the sequence of the row: 32-way search for the last s with q_offsets[s] <= row
   int low = 0, count = p.sequences;
+  bool found = true;
   while (count > 0) {
     const int stride = (count + 31) / 32;
     const bool reached = lane * stride < count && p.q_offsets[low + lane * stride] <= row;
     const unsigned votes = __ballot_sync(0xffffffffu, reached);
-    if (votes == 0) return;
+    if (votes == 0) {
+      found = false;
+      break;
+    }
     const int last = 31 - __clz(votes);
     const int behind = count - last * stride;
     low += last * stride;
@@ -306,30 +311,42 @@ __global__ void __launch_bounds__(256) packed_rows_join_kernel(const RowsParams 
   const int q0 = p.q_offsets[low], q1 = p.q_offsets[low + 1];
   const int k0 = p.k_offsets[low], k1 = p.k_offsets[low + 1];
   const int keys = p.k_lengths ? p.k_lengths[low] : k1 - k0;
-  if (row < q0 || row >= q1 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k || keys < 0 || keys > k1 - k0) return;
+  found = found && row >= q0 && row < q1 && q1 <= p.total_q && k0 >= 0 && k1 >= k0 && k1 <= p.total_k && keys >= 0 &&
+          keys <= k1 - k0;
   const int kv_head = head / p.group, in_group = head % p.group;
   const int piece = in_group / QROWS;
   const int heads = min(QROWS, p.group - piece * QROWS);
   const int chunks = (keys + p.chunk - 1) / p.chunk;
-  if (chunks <= 1 || (q1 - q0) * heads > QROWS) return;  // written by the first launch
+  after_previous_launch();
+  if (!found || chunks <= 1 || (q1 - q0) * heads > QROWS) return;  // written by the first launch
   const int f = (row - q0) * heads + in_group % QROWS;
-  const int64_t first = int64_t(k0) / p.chunk + low;
-  auto slot = [&](int c) { return (((first + c) * p.hkv + kv_head) * p.pieces + piece) * QROWS + f; };
+  const int64_t step = int64_t(p.hkv) * p.pieces * QROWS;
+  const int64_t first = ((int64_t(k0) / p.chunk + low) * p.hkv * p.pieces + kv_head * p.pieces + piece) * QROWS + f;
   float high = -INFINITY;
-  for (int c = lane; c < chunks; c += 32) high = fmaxf(high, p.part_lse[slot(c)]);
+  for (int c = lane; c < chunks; c += 32) high = fmaxf(high, p.part_lse[first + c * step]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.f;
 #pragma unroll 4
-  for (int c = 0; c < chunks; ++c) {
-    const float l = p.part_lse[slot(c)];
+  for (int c = warp; c < chunks; c += warps) {
+    const int64_t slot = first + c * step;
+    const float l = p.part_lse[slot];
     const float share = l == -INFINITY ? 0.f : exp2f(l - high);
     total += share;
     if (lane * 4 < p.dim) {
-      const float4 y = *reinterpret_cast<const float4*>(p.part_out + slot(c) * p.dim + lane * 4);
+      const float4 y = *reinterpret_cast<const float4*>(p.part_out + slot * p.dim + lane * 4);
       x.x += share * y.x; x.y += share * y.y; x.z += share * y.z; x.w += share * y.w;
     }
+  }
+  partial[warp][lane] = x;
+  if (lane == 0) weight[warp] = total;
+  __syncthreads();
+  if (warp != 0) return;
+  for (int w = 1; w < warps; ++w) {
+    const float4 y = partial[w][lane];
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    total += weight[w];
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   if (lane * 4 < p.dim)
@@ -345,14 +362,17 @@ cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
                                              rows_smem<DP>());
   if (e != cudaSuccess) return e;
   const int64_t grid = (p.total_k / p.chunk + p.sequences) * p.hkv * p.pieces;
-  const int64_t joins = (p.total_q * p.hq + 7) / 8;
+  const int64_t joins = p.total_q * p.hq;
   if (grid > 2147483647ll || joins > 2147483647ll) {
     set_error_detail("packed_attention: too many chunks for one launch");
     return cudaErrorInvalidValue;
   }
   packed_rows_kernel<DP, FP16><<<unsigned(grid), WARPS * 32, rows_smem<DP>(), stream>>>(p);
-  if (p.total_k > p.chunk) packed_rows_join_kernel<FP16><<<unsigned(joins), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  const cudaError_t launched = cudaGetLastError();
+  if (launched != cudaSuccess || p.total_k <= p.chunk) return launched;
+  const int64_t most = p.total_k / p.chunk + 1;  // chunks of a sequence
+  const int warps = most < JOIN_WARPS ? int(most) : JOIN_WARPS;
+  return launch_behind(packed_rows_join_kernel<FP16>, dim3(unsigned(joins)), warps * 32, 0, stream, p);
 }
 
 }  // namespace

@@ -13,6 +13,26 @@
 
 namespace agb {
 
+// A launch that may begin while the one before it still runs: its blocks take up what they can and wait
+// (after_previous_launch) before they read what that launch writes.  Every thread waits, so the
+// second launch never ends before the first.
+__device__ __forceinline__ void after_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(unsigned(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+
 struct PackedSpan {
   int unit_in_sequence;  // piece number within the sequence, or -1: none, or -2: rows behind the last sequence
   int sequence;
