@@ -2,8 +2,9 @@
 //
 //   s = scale q k^T over the visible keys (j <= i + keys - rows), p = softmax(s), out = p v
 //
-// Persistent CTAs, one an SM, work through items (piece of a sequence's queries, two score tiles, key
-// range) in the order of falling length, in a boustrophedon over the CTAs.  The two tiles of 128 rows
+// A CTA works through items (piece of a sequence's queries, two score tiles, key range), which come in the
+// order of falling length: it is launched for one and takes over further ones that have not started yet
+// (one CTA fits an SM).  The two tiles of 128 rows
 // are two query heads that share a key head, or, when a key head has an odd number of query heads,
 // two neighbouring tiles of one head; both read the same K and V tiles.
 //   warps 0-3  softmax of tile 0: one query row per thread; then its output
@@ -12,7 +13,7 @@
 //   warp 9     MMA issuer: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM (one elected thread in a
 //              branch of its own: a product then takes the pipe's 64 cycles, against 91 to 105 where
 //              the whole warp runs the loop and elects a lane for every instruction)
-//   warp 10    finds the items, one ahead
+//   warp 10    finds the items, up to two ahead
 //   warp 11    clears the V rows behind the last key, so that whatever lies there (another sequence,
 //              NaN) never meets a product
 // The third warpgroup hands registers to the other two.  While one tile is in its softmax the tensor
@@ -45,7 +46,7 @@ constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;  // 2 x 208 + 80 fit the laun
 constexpr uint32_t COL_S = 0, COL_O = 256;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int STAGE_BYTES = 32 * 64;  // a warp's part of the output on its way: 32 rows x 64 bytes
+constexpr int STAGE_BYTES = 32 * 128;  // a warp's part of the output on its way: 32 rows x 128 bytes
 
 template <int DP>
 constexpr int fwd_smem() {
@@ -65,7 +66,6 @@ struct FwdParams {
   int hq, dim, group, splits;
   int head_units;   // items side by side for one piece: hq / 2 (pairs of heads) or hq
   int paired;       // 1: the tiles are two heads, 0: two neighbouring row tiles
-  int64_t units;    // items, among them some without work
   float scale_log2;
   int* status;
 };
@@ -133,11 +133,14 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   uint64_t* s_full = bars + 10;    // [2 tiles] scores complete
   uint64_t* p_ready = bars + 12;   // [2 tiles][2 halves of the keys] probabilities in TMEM (count 4)
   uint64_t* o_done = bars + 16;    // [2 tiles] last product complete
-  uint64_t* v_ragged = bars + 18;  // an item's ragged last V tile is there
+  uint64_t* v_ragged = bars + 18;  // an item's ragged last V tile is on its way
   uint64_t* v_clean = bars + 19;   // and its rows behind the last key are cleared
   uint64_t* item_full = bars + 20; // [2]
   uint64_t* item_empty = bars + 22;  // [2] (count ITEM_READERS)
-  Item* items = reinterpret_cast<Item*>(bars + 24);  // [2]
+  uint64_t* answer_full = bars + 24;
+  uint64_t* item_loaded = bars + 25; // every load of an item is issued
+  uint64_t* answer = bars + 26;      // 16 bytes: the next block taken over
+  Item* items = reinterpret_cast<Item*>(bars + 28);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -163,6 +166,8 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
     mbar_init(v_ragged, 1);
     mbar_init(v_clean, 1);
+    mbar_init(answer_full, 1);
+    mbar_init(item_loaded, 1);
     mbar_fence_init();
   }
   if (warp == 9) {
@@ -195,10 +200,13 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const Item& it = items[i & 1];
           const int kind = it.kind, n = it.n, kv_head = it.kv_head, q0 = it.q0, row0 = it.k0 + it.lo * ROWS;
           const int head[2] = {it.head[0], it.head[1]}, first[2] = {it.first[0], it.first[1]};
-          const bool there[2] = {it.tiles[0] > 0, it.tiles[1] > 0};
+          const bool there[2] = {it.tiles[0] > 0, it.tiles[1] > 0}, ragged = it.last_valid < ROWS;
           item_free(i);
           if (kind == ITEM_END) break;
-          if (n == 0) continue;
+          if (n == 0) {
+            mbar_arrive(item_loaded);
+            continue;
+          }
           if (!mbar_wait(q_empty, (used & 1) ^ 1, guard, kTimeoutProducer)) { ok = false; break; }
           ++used;
           mbar_expect_tx(q_full, (there[0] + there[1]) * TILE_BYTES);
@@ -219,7 +227,9 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             mbar_expect_tx(&v_full[st], TILE_BYTES);
             for (int a = 0; a < ATOMS; ++a)
               tma_load_3d(sV + st * TILE_BYTES + a * HALF_BYTES, &tm_v, &v_full[st], a * 64, kv_head, row);
+            if (ragged && j + 1 == n) mbar_arrive(v_ragged);
           }
+          mbar_arrive(item_loaded);
         }
         if (!ok || *abort_flag) {
           // give in-flight copies time to land before shared memory is released
@@ -269,10 +279,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             const int st = (loads + j) % KV_STAGES, next = (loads + j + 1) % KV_STAGES;
             const bool more = j + 1 < n;
             if (!mbar_wait(&v_full[st], ((loads + j) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
-            if (!more && ragged) {
-              mbar_arrive(v_ragged);
-              if (!mbar_wait(v_clean, cleaned++ & 1, guard, kTimeoutMma)) { ok = false; break; }
-            }
+            if (!more && ragged && !mbar_wait(v_clean, cleaned++ & 1, guard, kTimeoutMma)) { ok = false; break; }
             if (more && !mbar_wait(&k_full[next], ((loads + j + 1) / KV_STAGES) & 1, guard, kTimeoutMma)) { ok = false; break; }
             const uint32_t v_addr = smem_u32(sV + st * TILE_BYTES);
 #pragma unroll
@@ -308,30 +315,37 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       __syncwarp();
     } else if (warp == 10) {
       // ------------------------------------------------------------------------ items
-      const int64_t ctas = gridDim.x;
-      int i = 0;
-      for (int64_t round = 0;; ++round) {
-        const int64_t unit = round * ctas + (round & 1 ? ctas - 1 - blockIdx.x : blockIdx.x);
-        const bool last = round * ctas >= p.units;
-        if (!last && unit >= p.units) continue;
+      // The next block is taken over once the last loads of the present item are issued, two key tiles
+      // before its end: earlier, and CTAs with long items would take blocks from those that are free.
+      uint32_t found = 0, asked = 0;
+      for (int64_t unit = blockIdx.x;;) {
+        const bool last = unit < 0;
         Item item{};
+        bool work = last;
         if (!last) {
-          const int split = int(unit % p.splits);
-          const int head_unit = int(unit / p.splits % p.head_units);
-          const PackedSpan span = find_piece(int(unit / p.splits / p.head_units), p.paired ? ROWS : 2 * ROWS, false,
-                                             p.q_offsets, p.k_offsets, p.k_lengths, p.sequences, p.total_q, p.total_k,
+          const int side = p.head_units * p.splits;  // blocks of one piece, splits fastest
+          const int piece = divide(int(unit), side), rest = int(unit) - piece * side;
+          const int head_unit = divide(rest, p.splits), split = rest - head_unit * p.splits;
+          const PackedSpan span = find_piece(piece, p.paired ? ROWS : 2 * ROWS, false, p.q_offsets, p.k_offsets,
+                                             p.k_lengths, p.sequences, p.total_q, p.total_k,
                                              head_unit == 0 && split == 0 ? p.status : nullptr);
-          if (span.unit_in_sequence == -1 || (span.unit_in_sequence == -2 && span.rows == 0)) continue;
-          item = make_item(span, p, head_unit, split);
+          work = !(span.unit_in_sequence == -1 || (span.unit_in_sequence == -2 && span.rows == 0));
+          if (work) item = make_item(span, p, head_unit, split);
         }
-        if (!mbar_wait_w(&item_empty[i & 1], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer)) break;
-        if (lane == 0) {
-          items[i & 1] = item;
-          mbar_arrive(&item_full[i & 1]);
+        if (work) {
+          if (!mbar_wait_w(&item_empty[found & 1], ((found >> 1) & 1) ^ 1, guard, kTimeoutProducer)) break;
+          if (lane == 0) {
+            items[found & 1] = item;
+            mbar_arrive(&item_full[found & 1]);
+          }
+          __syncwarp();
+          if (last || !mbar_wait_w(item_loaded, found & 1, guard, kTimeoutProducer)) break;
+          ++found;
         }
+        if (lane == 0) steal(smem_u32(answer), answer_full);
+        if (!mbar_wait_w(answer_full, asked++ & 1, guard, kTimeoutProducer)) break;
+        unit = stolen(smem_u32(answer));
         __syncwarp();
-        if (last) break;
-        ++i;
       }
     } else {
       // ------------------------------------------------------------- rows behind the keys
@@ -345,12 +359,13 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (n == 0) continue;
         loads += n;
         if (valid >= ROWS) continue;
-        if (!mbar_wait_w(v_ragged, cleaned++ & 1, guard, kTimeoutProducer)) break;
-        // a row is 128 bytes of each atom whatever the swizzle, which permutes within the row
-        uint8_t* tile = sV + ((loads - 1) % KV_STAGES) * TILE_BYTES;
-        for (int w = valid * 8 + lane; w < ROWS * 8; w += 32)
-          for (int a = 0; a < ATOMS; ++a)
-            *reinterpret_cast<uint4*>(tile + a * HALF_BYTES + w * 16) = make_uint4(0, 0, 0, 0);
+        // Once that load is issued its stage's barrier is in the phase of this tile, and stays there
+        // until the rows are cleared: its parity then says whether the tile has arrived.
+        const int st = (loads - 1) % KV_STAGES;
+        if (!mbar_wait_w(v_ragged, cleaned++ & 1, guard, kTimeoutProducer) ||
+            !mbar_wait_w(&v_full[st], ((loads - 1) / KV_STAGES) & 1, guard, kTimeoutProducer))
+          break;
+        clear_rows<ATOMS>(smem_u32(sV + st * TILE_BYTES), valid, lane);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_clean);
@@ -365,7 +380,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int my_row = quarter * 32 + lane;
     const uint32_t col_s = tmem_base + lane_base + COL_S + t * 128;
     const uint32_t col_o = tmem_base + lane_base + COL_O + t * 128;
-    uint8_t* stage = sOut + warp * STAGE_BYTES;
+    const uint32_t stage = smem_u32(sOut + warp * STAGE_BYTES);
     bool ok = true;
     uint32_t done = 0, outs = 0;                 // score blocks and outputs of earlier items
     for (int i = 0; ok; ++i) {
@@ -373,10 +388,11 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const Item& it = items[i & 1];
       const int kind = it.kind, my_tiles = it.tiles[t], my_rows = it.rows[t], my_head = it.head[t], split = it.split;
       const int q_row = it.q0 + it.first[t];     // first row of the tile
-      // keys that this row and the tile's first row see, from the first key of the range on
-      const int before = it.keys - it.query_rows + it.first[t] + 1 - it.lo * ROWS;
-      const int seen = min(it.keys - it.lo * ROWS, before + my_row);
-      const int seen_first = min(it.keys - it.lo * ROWS, before);
+      // keys that this row, and the warp's first row, see, from the first key of the range on
+      const int it_keys = it.keys - it.lo * ROWS;
+      const int before = it_keys - it.query_rows + it.first[t] + 1;
+      const int seen = min(it_keys, before + my_row);
+      const int seen_warp = min(it_keys, before + quarter * 32);
       const int uncovered0 = it.q0, uncovered = it.query_rows;
       __syncwarp();
       if (lane == 0) item_free(i);
@@ -400,14 +416,20 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(col_s + c * 32, s[c]);
         tmem_ld_wait();
-        const bool masked = seen_first < (j + 1) * ROWS;  // the diagonal and the ragged last tile
+        // Only the diagonal and the ragged last tile mask.  There, of the 32 keys of chunk c, every row of
+        // the warp sees all (32 c + 32 <= sure), or none (32 c >= most), or the rows differ; all these
+        // tests are uniform over the warp.
+        const int sure = seen_warp - j * ROWS;
+        const bool masked = sure < ROWS;
         if (masked) {
           const int valid = seen - j * ROWS;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 + 32 <= sure) continue;
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (c * 32 + k >= valid) s[c][k] = 0xff800000u;  // -inf
+          }
         }
         float m4[4];
 #pragma unroll
@@ -447,27 +469,46 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         // One pair of unmasked scores in four takes the exponential of the FMA pipe: a tile's share of
         // the special-function unit (16 a cycle) is as long as its products.  1661 us against 1690
         // without, 1708 for one in eight and 1747 for three in eight, at 16384 tokens.
-        auto probabilities = [&](auto all) {
+        auto chunk = [&](const uint32_t (&x32)[32], uint32_t* to, auto all) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 x = ffma2(make_float2(__uint_as_float(x32[2 * k]), __uint_as_float(x32[2 * k + 1])), scale2, shift2);
+            const float2 e = decltype(all)::value && k % 4 == 3 ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
+            sums[k & 3] = fadd2(sums[k & 3], e);
+            to[k] = pack16<FP16>(e.x, e.y);
+          }
+        };
+        auto hand_over = [&](const uint32_t (&packed)[32], int c) {
+          tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
+        };
+        if (!masked) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t packed[32];
+            chunk(s[2 * c], packed, std::true_type{});
+            chunk(s[2 * c + 1], packed + 16, std::true_type{});
+            hand_over(packed, c);
+          }
+        } else {
+          const int most = min(it_keys - j * ROWS, sure + 31);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t packed[32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const uint32_t* src = &s[2 * c + (k >> 4)][(2 * k) & 31];  // columns 2k, 2k+1 of half c
-              const float2 x = ffma2(make_float2(__uint_as_float(src[0]), __uint_as_float(src[1])), scale2, shift2);
-              const float2 e = decltype(all)::value && k % 4 == 3 ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
-              sums[k & 3] = fadd2(sums[k & 3], e);
-              packed[k] = pack16<FP16>(e.x, e.y);
+            for (int h = 0; h < 2; ++h) {
+              if ((2 * c + h) * 32 + 32 <= sure) chunk(s[2 * c + h], packed + 16 * h, std::true_type{});
+              else if ((2 * c + h) * 32 < most) chunk(s[2 * c + h], packed + 16 * h, std::false_type{});
+              else
+#pragma unroll
+                for (int k = 0; k < 16; ++k) packed[16 * h + k] = 0;
             }
-            tmem_st_32x32(col_s + c * 32, packed);  // over the scores, which are in registers
-            tmem_st_wait();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[2 * t + c]);
+            hand_over(packed, c);
           }
-        };
-        if (masked) probabilities(std::false_type{});
-        else probabilities(std::true_type{});
+        }
         const float2 sum2 = fadd2(fadd2(sums[0], sums[1]), fadd2(sums[2], sums[3]));
         l_sum += sum2.x + sum2.y;
       }
@@ -482,56 +523,66 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int64_t row = int64_t(q_row) + quarter * 32;  // its first
       const int64_t at = (partial ? int64_t(split) * p.total_q : 0) * p.hq + row * p.hq + my_head;
       if (live > 0 && !(partial && my_tiles == 0)) {
-        // 64 bytes of every row at a time through shared memory, words permuted against bank conflicts:
-        // one row a thread would make a store touch 32 lines
-        uint8_t* put = stage + lane * 64;
-        const int flip = (lane >> 1) & 3;
-        auto flush = [&](uint8_t* dst, int64_t pitch, int bytes) {  // `bytes` left of a row from this chunk on
+        // 128 bytes of every row at a time through shared memory (64 elements, or 32 of a partial
+        // result), words permuted against bank conflicts: stores of one row a thread would touch 32
+        // lines each.
+        const uint32_t put = stage + lane * 128;
+        auto flush = [&](uint8_t* dst, int64_t pitch, int bytes) {  // `bytes` left of a row from here on
           __syncwarp();
+          const int w = lane & 7;
+          uint4 v[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = k * 8 + (lane >> 2), w = lane & 3;
-            if (r < live && w * 16 < bytes)
-              *reinterpret_cast<uint4*>(dst + r * pitch + w * 16) =
-                  *reinterpret_cast<const uint4*>(stage + r * 64 + (w ^ ((r >> 1) & 3)) * 16);
+          for (int k = 0; k < 8; ++k) v[k] = get16(stage + (k * 4 + (lane >> 3)) * 128 + (w ^ ((k * 4 + (lane >> 3)) & 7)) * 16);
+          if (w * 16 < bytes) {
+            uint8_t* to = dst + (lane >> 3) * pitch + w * 16;
+            if (live == 32) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k, to += 4 * pitch) store16(to, v[k]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k, to += 4 * pitch)
+                if (k * 4 + (lane >> 3) < live) store16(to, v[k]);
+            }
           }
           __syncwarp();
         };
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          if (c * 32 >= p.dim) break;
-          uint32_t o[32];
-          if (my_tiles > 0) {
-            tmem_ld_32x32(col_o + c * 32, o);
-            tmem_ld_wait();
-          } else {
+        for (int c = 0; c < DP / 64; ++c) {
+          uint32_t o[2][32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = 0;
+          for (int h = 0; h < 2; ++h) {
+            if (my_tiles > 0) tmem_ld_32x32(col_o + c * 64 + h * 32, o[h]);
+            else
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[h][k] = 0;
           }
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+          tmem_ld_wait();
           if (partial) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<uint4*>(put + (g ^ flip) * 16) =
-                    make_uint4(o[h * 16 + g * 4], o[h * 16 + g * 4 + 1], o[h * 16 + g * 4 + 2], o[h * 16 + g * 4 + 3]);
-              flush(reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 32 + h * 16), int64_t(p.hq) * p.dim * 4,
-                    (p.dim - c * 32 - h * 16) * 4);
+              for (int g = 0; g < 8; ++g)
+                put16(put + (g ^ (lane & 7)) * 16,
+                      make_uint4(__float_as_uint(__uint_as_float(o[h][g * 4 + 0]) * inv),
+                                 __float_as_uint(__uint_as_float(o[h][g * 4 + 1]) * inv),
+                                 __float_as_uint(__uint_as_float(o[h][g * 4 + 2]) * inv),
+                                 __float_as_uint(__uint_as_float(o[h][g * 4 + 3]) * inv)));
+              flush(reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 64 + h * 32), int64_t(p.hq) * p.dim * 4,
+                    (p.dim - c * 64 - h * 32) * 4);
             }
           } else {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < 8; ++g) {
+              const uint32_t* x = &o[g >> 2][(g & 3) * 8];
               uint4 v;
-              v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]), __uint_as_float(o[g * 8 + 1]));
-              v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]), __uint_as_float(o[g * 8 + 3]));
-              v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]), __uint_as_float(o[g * 8 + 5]));
-              v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]), __uint_as_float(o[g * 8 + 7]));
-              *reinterpret_cast<uint4*>(put + (g ^ flip) * 16) = v;
+              v.x = pack16<FP16>(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
+              v.y = pack16<FP16>(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
+              v.z = pack16<FP16>(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
+              v.w = pack16<FP16>(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
+              put16(put + (g ^ (lane & 7)) * 16, v);
             }
-            flush(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 32), int64_t(p.hq) * p.dim * 2,
-                  (p.dim - c * 32) * 2);
+            flush(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 64), int64_t(p.hq) * p.dim * 2,
+                  (p.dim - c * 64) * 2);
           }
         }
       }
@@ -610,14 +661,13 @@ cudaError_t launch_tiles(const PackedArgs& a, const CUtensorMap& tq, const CUten
   p.scale_log2 = a.scale * LOG2E;
   p.status = a.status;
   const int step = p.paired ? ROWS : 2 * ROWS;
-  p.units = (a.total_q / step + a.sequences + 1) * p.head_units * p.splits;
+  const int64_t units = (a.total_q / step + a.sequences + 1) * p.head_units * p.splits;
   const int64_t blocks = (a.total_q * a.hq + 7) / 8;
-  if (blocks > 2147483647ll) {
+  if (units > 2147483647ll || blocks > 2147483647ll) {
     set_error_detail("packed_attention: too many rows for one launch");
     return cudaErrorInvalidValue;
   }
-  const unsigned grid = unsigned(p.units < a.sm_count ? p.units : a.sm_count);
-  packed_tiles_kernel<DP, FP16><<<grid, FWD_THREADS, fwd_smem<DP>(), stream>>>(tq, tk, tv, p);
+  packed_tiles_kernel<DP, FP16><<<unsigned(units), FWD_THREADS, fwd_smem<DP>(), stream>>>(tq, tk, tv, p);
   const cudaError_t launched = cudaGetLastError();
   if (launched != cudaSuccess || a.splits == 1) return launched;
   return launch_behind(packed_join_kernel<FP16>, dim3(unsigned(blocks)), 256, 0, stream, a.part_out, a.part_lse,

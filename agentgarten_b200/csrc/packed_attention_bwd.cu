@@ -48,13 +48,6 @@ struct BwdParams {
   int* status;
 };
 
-// Clears rows [from, 128) of a tile (ATOMS blocks of 128 rows x 128 bytes); converged warp.
-template <int ATOMS>
-__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
-  for (int i = from * 8 + lane; i < ROWS * 8; i += 32)
-    for (int a = 0; a < ATOMS; ++a) *reinterpret_cast<uint4*>(tile + a * HALF_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-}
-
 template <int ATOMS>
 __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map, uint64_t* bar, int head, int row) {
   for (int a = 0; a < ATOMS; ++a) tma_load_3d(tile + a * HALF_BYTES, map, bar, a * 64, head, row);
@@ -205,8 +198,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         ok = mbar_wait_w(&k_full[st], parity, guard, kTimeoutProducer) &&
              mbar_wait_w(&v_full[st], parity, guard, kTimeoutProducer);
         if (ok) {
-          clear_rows<ATOMS>(sK + st * TILE_BYTES, last_valid, lane);
-          clear_rows<ATOMS>(sV + st * TILE_BYTES, last_valid, lane);
+          clear_rows<ATOMS>(smem_u32(sK + st * TILE_BYTES), last_valid, lane);
+          clear_rows<ATOMS>(smem_u32(sV + st * TILE_BYTES), last_valid, lane);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(clean);
@@ -501,8 +494,8 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (ragged) {
             ok = mbar_wait_w(&qd_full[st], (i >> 1) & 1, guard, kTimeoutProducer);
             if (!ok) break;
-            clear_rows<ATOMS>(sQ + st * TILE_BYTES, tail_rows, lane);
-            clear_rows<ATOMS>(sdO + st * TILE_BYTES, tail_rows, lane);
+            clear_rows<ATOMS>(smem_u32(sQ + st * TILE_BYTES), tail_rows, lane);
+            clear_rows<ATOMS>(smem_u32(sdO + st * TILE_BYTES), tail_rows, lane);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&qd_clean[st]);

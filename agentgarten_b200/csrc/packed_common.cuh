@@ -13,6 +13,31 @@
 
 namespace agb {
 
+// 16-byte accesses of shared memory by its own addresses (through a pointer that was aligned by hand the
+// compiler only sees generic memory: clearing a tile's rows took five times as long).
+__device__ __forceinline__ void put16(uint32_t address, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 get16(uint32_t address) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store16(void* to, uint4 v) {
+  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};"
+               ::"l"(__cvta_generic_to_global(to)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Clears rows [from, 128) of a tile (ATOMS blocks of 128 rows x 128 bytes; a row is 128 bytes of each
+// block whatever the swizzle, which permutes within the row); converged warp.
+template <int ATOMS>
+__device__ __forceinline__ void clear_rows(uint32_t tile, int from, int lane) {
+#pragma unroll 4
+  for (int i = from * 8 + lane; i < 128 * 8; i += 32)
+#pragma unroll
+    for (int a = 0; a < ATOMS; ++a) put16(tile + a * 16384 + i * 16, make_uint4(0, 0, 0, 0));
+}
+
 // A launch that may begin while the one before it still runs: its blocks take up what they can and wait
 // (after_previous_launch) before they read what that launch writes.  Every thread waits, so the
 // second launch never ends before the first.
@@ -31,6 +56,38 @@ cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, int threads, siz
   config.attrs = &attribute;
   config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+
+// Work of a block that has not started yet, taken over by a running one (cluster launch control): the
+// hardware's own queue in place of a counter in memory.  `steal` asks, `stolen` reads the answer once
+// `bar` has it (16 bytes): the number of the block taken over, or -1 when none is left (do not ask again).
+__device__ __forceinline__ void steal(uint32_t answer, uint64_t* bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(answer), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int64_t stolen(uint32_t answer) {
+  uint32_t block = 0, taken = 0;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n\t}"
+      : "+r"(block), "=r"(taken) : "r"(answer) : "memory");
+  // the answer is read before the next one may be written over it
+  fence_proxy_async_smem();
+  return taken ? int64_t(block) : -1;
+}
+
+// a / b of non-negative a and positive b: an estimate in 32-bit floating point, put right in integers (the
+// compiler's own division takes a few hundred cycles before the first load of a block).
+__device__ __forceinline__ int divide(int a, int b) {
+  int q = int(__fdividef(float(a), float(b)));
+  int r = a - q * b;
+  while (r < 0) { --q; r += b; }
+  while (r >= b) { ++q; r -= b; }
+  return q;
 }
 
 struct PackedSpan {
@@ -107,15 +164,16 @@ constexpr int MAX_RANKED = 64;
 
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
+template <int R>  // sequences <= 32 R
 __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const int* __restrict__ q_offsets,
                                          const int* __restrict__ k_offsets, const int* __restrict__ k_lengths,
                                          int sequences, int64_t total_q, int64_t total_k, int* status) {
   const int lane = threadIdx.x & 31;
-  int q0[2], q1[2], k0[2], k1[2], keys[2], count[2], most[2], cap[2];
+  int q0[R], q1[R], k0[R], k1[R], keys[R], count[R], most[R], cap[R];
   bool bad = false;
   const int end = (by_keys ? k_offsets : q_offsets)[sequences];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int s = lane + 32 * i;
     const bool there = s < sequences;
     const int at = there ? s : 0;
@@ -126,7 +184,7 @@ __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const
     keys[i] = there && k_lengths ? k_lengths[at] : k1[i] - k0[i];
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int rows = q1[i] - q0[i];
     const bool fits = q0[i] >= 0 && rows >= 0 && q1[i] <= total_q && k0[i] >= 0 && k1[i] >= k0[i] &&
                       k1[i] <= total_k && keys[i] >= 0 && keys[i] <= k1[i] - k0[i];
@@ -143,7 +201,13 @@ __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0 && status) atomicCAS(status, 0, kBadIndex);
   PackedSpan span{-1, 0, 0, 0, 0, 0, 0};
-  const int all = warp_sum(count[0] + count[1]);
+  auto sum_of = [&](auto of_register) {
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) sum += of_register(i);
+    return warp_sum(sum);
+  };
+  const int all = sum_of([&](int i) { return count[i]; });
   if (rank >= all) {
     const int64_t total = by_keys ? total_k : total_q;
     if (end < 0 || end > total) return span;
@@ -159,9 +223,19 @@ __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const
     const int n = most[i] - length + 1;
     return length > cap[i] || n < 0 ? 0 : (n < count[i] ? n : count[i]);
   };
+  if (sequences == 1) {
+    const int piece = by_keys ? rank : count[0] - 1 - rank;
+    span.unit_in_sequence = __shfl_sync(0xffffffffu, piece, 0);
+    span.q0 = __shfl_sync(0xffffffffu, q0[0], 0);
+    span.rows = __shfl_sync(0xffffffffu, q1[0], 0) - span.q0;
+    span.k0 = __shfl_sync(0xffffffffu, k0[0], 0);
+    span.room = __shfl_sync(0xffffffffu, k1[0], 0) - span.k0;
+    span.keys = __shfl_sync(0xffffffffu, keys[0], 0);
+    return span;
+  }
   int low = 0x7fffffff, high = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < R; ++i)
     if (count[i] > 0) {
       low = min(low, min(cap[i], most[i] - count[i] + 1));
       high = max(high, cap[i]);
@@ -170,19 +244,19 @@ __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const
   high = __reduce_max_sync(0xffffffffu, high) + 1;  // nothing is this long
   while (high - low > 1) {  // the greatest length that more than `rank` pieces reach
     const int middle = low + (high - low) / 2;
-    if (warp_sum(longer(0, middle) + longer(1, middle)) > rank) low = middle;
+    if (sum_of([&](int i) { return longer(i, middle); }) > rank) low = middle;
     else high = middle;
   }
   // the pieces of exactly this length, sequence by sequence
-  int behind[2], here[2];
+  int behind[R], here[R];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     behind[i] = longer(i, low + 1);
     here[i] = longer(i, low) - behind[i];
   }
-  int index = rank - warp_sum(behind[0] + behind[1]);
+  int index = rank - sum_of([&](int i) { return behind[i]; });
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     int before = here[i];  // inclusive sum over the lanes
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -213,8 +287,10 @@ __device__ inline PackedSpan find_ranked(int rank, int step, bool by_keys, const
 __device__ __forceinline__ PackedSpan find_piece(int unit, int step, bool by_keys, const int* __restrict__ q_offsets,
                                                  const int* __restrict__ k_offsets, const int* __restrict__ k_lengths,
                                                  int sequences, int64_t total_q, int64_t total_k, int* status) {
+  if (sequences <= 32)
+    return find_ranked<1>(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
   if (sequences <= MAX_RANKED)
-    return find_ranked(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
+    return find_ranked<2>(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
   PackedSpan span = find_unit(unit, step, by_keys, q_offsets, k_offsets, k_lengths, sequences, total_q, total_k, status);
   if (!by_keys && span.unit_in_sequence >= 0) {  // late pieces of a sequence see the most keys and come first
     const int pieces = (span.rows + step - 1) / step;
