@@ -523,29 +523,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int64_t row = int64_t(q_row) + quarter * 32;  // its first
       const int64_t at = (partial ? int64_t(split) * p.total_q : 0) * p.hq + row * p.hq + my_head;
       if (live > 0 && !(partial && my_tiles == 0)) {
-        // 128 bytes of every row at a time through shared memory (64 elements, or 32 of a partial
-        // result), words permuted against bank conflicts: stores of one row a thread would touch 32
-        // lines each.
-        const uint32_t put = stage + lane * 128;
-        auto flush = [&](uint8_t* dst, int64_t pitch, int bytes) {  // `bytes` left of a row from here on
-          __syncwarp();
-          const int w = lane & 7;
-          uint4 v[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = get16(stage + (k * 4 + (lane >> 3)) * 128 + (w ^ ((k * 4 + (lane >> 3)) & 7)) * 16);
-          if (w * 16 < bytes) {
-            uint8_t* to = dst + (lane >> 3) * pitch + w * 16;
-            if (live == 32) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k, to += 4 * pitch) store16(to, v[k]);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 8; ++k, to += 4 * pitch)
-                if (k * 4 + (lane >> 3) < live) store16(to, v[k]);
-            }
-          }
-          __syncwarp();
-        };
+        // 128 bytes of every row at a time: 64 elements, or 32 of a partial result
 #pragma unroll 1
         for (int c = 0; c < DP / 64; ++c) {
           uint32_t o[2][32];
@@ -562,13 +540,13 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
               for (int g = 0; g < 8; ++g)
-                put16(put + (g ^ (lane & 7)) * 16,
+                put16(stage_word(stage, lane, g),
                       make_uint4(__float_as_uint(__uint_as_float(o[h][g * 4 + 0]) * inv),
                                  __float_as_uint(__uint_as_float(o[h][g * 4 + 1]) * inv),
                                  __float_as_uint(__uint_as_float(o[h][g * 4 + 2]) * inv),
                                  __float_as_uint(__uint_as_float(o[h][g * 4 + 3]) * inv)));
-              flush(reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 64 + h * 32), int64_t(p.hq) * p.dim * 4,
-                    (p.dim - c * 64 - h * 32) * 4);
+              flush_rows(stage, reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 64 + h * 32),
+                         int64_t(p.hq) * p.dim * 4, (p.dim - c * 64 - h * 32) * 4, live, lane);
             }
           } else {
 #pragma unroll
@@ -579,10 +557,10 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               v.y = pack16<FP16>(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
               v.z = pack16<FP16>(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
               v.w = pack16<FP16>(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
-              put16(put + (g ^ (lane & 7)) * 16, v);
+              put16(stage_word(stage, lane, g), v);
             }
-            flush(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 64), int64_t(p.hq) * p.dim * 2,
-                  (p.dim - c * 64) * 2);
+            flush_rows(stage, reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 64),
+                       int64_t(p.hq) * p.dim * 2, (p.dim - c * 64) * 2, live, lane);
           }
         }
       }

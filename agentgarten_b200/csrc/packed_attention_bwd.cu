@@ -20,6 +20,8 @@
 #include "packed_common.cuh"
 #include "tensormap.h"
 
+#include <type_traits>
+
 namespace agb {
 
 bool make_packed_map(CUtensorMap* map, const void* base, int dim, int heads, int64_t rows, int64_t head_stride,
@@ -53,41 +55,53 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
   for (int a = 0; a < ATOMS; ++a) tma_load_3d(tile + a * HALF_BYTES, map, bar, a * 64, head, row);
 }
 
-// Writes a warp's 32 rows of an FP32 accumulator, scaled and rounded.  Without `filled` (uniform over
-// the warp) the accumulator holds nothing and zeros are written; so are the rows that are not `live`.
-template <int DP, bool FP16>
-__device__ __forceinline__ void store_rows(uint16_t* dst, uint32_t taddr, int dim, float scale, bool row_ok, bool filled,
-                                           bool live, int c0, int c1) {
-#pragma unroll 1
-  for (int c = c0; c < c1; ++c) {
-    uint32_t o[32];
-    if (filled) {
-      tmem_ld_32x32(taddr + c * 32, o);
-      tmem_ld_wait();
-    }
-    if (!filled || !live) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = 0;
-    }
-    if (row_ok) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint4 v;
-        v.x = pack16<FP16>(__uint_as_float(o[g * 8 + 0]) * scale, __uint_as_float(o[g * 8 + 1]) * scale);
-        v.y = pack16<FP16>(__uint_as_float(o[g * 8 + 2]) * scale, __uint_as_float(o[g * 8 + 3]) * scale);
-        v.z = pack16<FP16>(__uint_as_float(o[g * 8 + 4]) * scale, __uint_as_float(o[g * 8 + 5]) * scale);
-        v.w = pack16<FP16>(__uint_as_float(o[g * 8 + 6]) * scale, __uint_as_float(o[g * 8 + 7]) * scale);
-        if (c * 32 + g * 8 < dim) *reinterpret_cast<uint4*>(dst + c * 32 + g * 8) = v;
-      }
-    }
+// Writes 64 columns of a warp's 32 rows of an FP32 accumulator, scaled and rounded, through its 4 KB of
+// stage.  Without `filled` (uniform over the warp) the accumulator holds nothing and zeros are
+// written; so are the rows that are not `live`.
+template <bool FP16>
+__device__ __forceinline__ void store_columns(uint16_t* dst, int64_t pitch, uint32_t taddr, int left, float scale, int rows,
+                                              bool filled, bool live, uint32_t stage, int lane) {
+  uint32_t o[2][32];
+  if (filled) {
+    tmem_ld_32x32(taddr, o[0]);
+    tmem_ld_32x32(taddr + 32, o[1]);
+    tmem_ld_wait();
   }
+  if (!filled || !live) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[h][i] = 0;
+  }
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    const uint32_t* x = &o[g >> 2][(g & 3) * 8];
+    uint4 v;
+    v.x = pack16<FP16>(__uint_as_float(x[0]) * scale, __uint_as_float(x[1]) * scale);
+    v.y = pack16<FP16>(__uint_as_float(x[2]) * scale, __uint_as_float(x[3]) * scale);
+    v.z = pack16<FP16>(__uint_as_float(x[4]) * scale, __uint_as_float(x[5]) * scale);
+    v.w = pack16<FP16>(__uint_as_float(x[6]) * scale, __uint_as_float(x[7]) * scale);
+    put16(stage_word(stage, lane, g), v);
+  }
+  flush_rows(stage, reinterpret_cast<uint8_t*>(dst), pitch * 2, left * 2, rows, lane);
 }
 
+// Probabilities of a pair of scores, one pair in four on the FMA pipe (see exp2_fma).
+template <bool FMA>
+__device__ __forceinline__ float2 exp2_pair(float2 x) {
+  return FMA ? exp2_fma(x) : make_float2(exp2f(x.x), exp2f(x.y));
+}
+
+// Seven tiles fill an SM (the ring of the operand that two products use has three stages, so that its
+// next load is on its way while the later product runs; with two, every second tile waited for it).
+// At least half of an SM's shared memory: two CTAs do not fit in its tensor memory.
+constexpr int RING = 3;
 template <int DP>
-constexpr int bwd_smem() {  // at least half of an SM's shared memory: two CTAs do not fit in its tensor memory
-  const int bytes = 6 * (DP / 64) * HALF_BYTES + 4 * ROWS * 4 + 1024 + 512;
+constexpr int bwd_smem() {
+  const int bytes = 7 * (DP / 64) * HALF_BYTES + 4 * ROWS * 4 + 384;
   return bytes > 120 * 1024 ? bytes : 120 * 1024;
 }
+static_assert(bwd_smem<128>() <= 232448, "an SM's shared memory");
 
 // ------------------------------------------------------------------------------- dQ
 // Products are issued one tile staggered: S(j+1) = Q K^T | dQ += dS(j) K | dP(j+1) = dO V^T.  The
@@ -101,25 +115,24 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                  const BwdParams p) {
   constexpr int ATOMS = DP / 64;
   constexpr int TILE_BYTES = ATOMS * HALF_BYTES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // the swizzle counts addresses in blocks of 1024 bytes
   uint8_t* sQ = smem;
   uint8_t* sdO = smem + TILE_BYTES;
-  uint8_t* sK = smem + 2 * TILE_BYTES;
-  uint8_t* sV = smem + 4 * TILE_BYTES;
-  float* halves = reinterpret_cast<float*>(smem + 6 * TILE_BYTES);  // [2][128] parts of delta
-  uint64_t* bars = reinterpret_cast<uint64_t*>(halves + 4 * ROWS);
+  uint8_t* sK = smem + 2 * TILE_BYTES;  // [RING]
+  uint8_t* sV = smem + 5 * TILE_BYTES;  // [2]
+  float* deltas = reinterpret_cast<float*>(smem + 7 * TILE_BYTES);  // [128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(deltas + 4 * ROWS);
   uint64_t* q_full = bars;        // Q and dO
-  uint64_t* k_full = bars + 1;    // [2]
-  uint64_t* v_full = bars + 3;    // [2]
-  uint64_t* k_empty = bars + 5;   // [2]
-  uint64_t* v_empty = bars + 7;   // [2]
-  uint64_t* s_full = bars + 9;    // [2] S of a tile is in TMEM
-  uint64_t* dp_full = bars + 11;  // dP of a tile is in TMEM
-  uint64_t* ds_ready = bars + 12; // [2] dS of key chunk c of both halves written over dP (count 8)
-  uint64_t* dq_done = bars + 14;  // every dQ product finished
-  uint64_t* clean = bars + 15;    // rows of the last K and V tile behind the last key cleared
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  uint64_t* k_full = bars + 1;    // [RING]
+  uint64_t* k_empty = bars + 4;   // [RING]
+  uint64_t* v_full = bars + 7;    // [2]
+  uint64_t* v_empty = bars + 9;   // [2]
+  uint64_t* s_full = bars + 11;   // [2] S of a tile is in TMEM
+  uint64_t* dp_full = bars + 13;  // dP of a tile is in TMEM
+  uint64_t* ds_ready = bars + 14; // [2] dS of key chunk c of both halves written over dP (count 8)
+  uint64_t* dq_done = bars + 16;  // every dQ product finished
+  uint64_t* clean = bars + 17;    // rows of the last K and V tile behind the last key cleared
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
 
@@ -142,10 +155,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     mbar_init(&ds_ready[1], 8);
     mbar_init(dq_done, 1);
     mbar_init(clean, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RING; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&v_full[i], 1);
       mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
     }
@@ -180,26 +195,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         load_tile<ATOMS>(sQ, &tm_q, q_full, head, q_row);
         load_tile<ATOMS>(sdO, &tm_do, q_full, head, q_row);
         for (int j = 0; j < n_tiles && ok; ++j) {
-          const int st = j & 1;
-          const uint32_t parity = ((j >> 1) & 1) ^ 1;
-          // the V stage comes free one product earlier than the K stage
-          if (!mbar_wait(&v_empty[st], parity, guard, kTimeoutProducer)) { ok = false; break; }
-          mbar_expect_tx(&v_full[st], TILE_BYTES);
-          load_tile<ATOMS>(sV + st * TILE_BYTES, &tm_v, &v_full[st], kv_head, span.k0 + j * ROWS);
-          if (!mbar_wait(&k_empty[st], parity, guard, kTimeoutProducer)) { ok = false; break; }
+          const int st = j % RING, sv = j & 1;
+          if (!mbar_wait(&k_empty[st], ((j / RING) & 1) ^ 1, guard, kTimeoutProducer)) { ok = false; break; }
           mbar_expect_tx(&k_full[st], TILE_BYTES);
           load_tile<ATOMS>(sK + st * TILE_BYTES, &tm_k, &k_full[st], kv_head, span.k0 + j * ROWS);
+          if (!mbar_wait(&v_empty[sv], ((j >> 1) & 1) ^ 1, guard, kTimeoutProducer)) { ok = false; break; }
+          mbar_expect_tx(&v_full[sv], TILE_BYTES);
+          load_tile<ATOMS>(sV + sv * TILE_BYTES, &tm_v, &v_full[sv], kv_head, span.k0 + j * ROWS);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       if (ragged && ok) {
-        const int st = (n_tiles - 1) & 1;
-        const uint32_t parity = ((n_tiles - 1) >> 1) & 1;
-        ok = mbar_wait_w(&k_full[st], parity, guard, kTimeoutProducer) &&
-             mbar_wait_w(&v_full[st], parity, guard, kTimeoutProducer);
+        const int j = n_tiles - 1, st = j % RING, sv = j & 1;
+        ok = mbar_wait_w(&k_full[st], (j / RING) & 1, guard, kTimeoutProducer) &&
+             mbar_wait_w(&v_full[sv], (j >> 1) & 1, guard, kTimeoutProducer);
         if (ok) {
           clear_rows<ATOMS>(smem_u32(sK + st * TILE_BYTES), last_valid, lane);
-          clear_rows<ATOMS>(smem_u32(sV + st * TILE_BYTES), last_valid, lane);
+          clear_rows<ATOMS>(smem_u32(sV + sv * TILE_BYTES), last_valid, lane);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(clean);
@@ -220,18 +232,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       // S of tile j into buffer j & 1 (its last reader, the exponentials of tile j - 2, finished
       // before dS(j-2) was announced, which the dQ product of that tile waited for).
       auto score_s = [&](int j) -> bool {
-        const int st = j & 1;
-        if (!mbar_wait(&k_full[st], (j >> 1) & 1, guard, kTimeoutMma)) return false;
+        const int st = j % RING;
+        if (!mbar_wait(&k_full[st], (j / RING) & 1, guard, kTimeoutMma)) return false;
         if (ragged && j == n_tiles - 1 && !mbar_wait(clean, 0, guard, kTimeoutMma)) return false;
         tc_fence_after_sync();
         const uint32_t k_addr = smem_u32(sK + st * TILE_BYTES);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-          tc_mma_ss(tmem_base + C_S + st * 128, make_smem_desc(q_addr + off, 16, 1024),
+          tc_mma_ss(tmem_base + C_S + (j & 1) * 128, make_smem_desc(q_addr + off, 16, 1024),
                       make_smem_desc(k_addr + off, 16, 1024), idesc_kk, kk != 0);
         }
-        tc_commit(&s_full[st]);
+        tc_commit(&s_full[j & 1]);
         return true;
       };
       // dP of tile j over dS(j-1), behind the dQ product that read it.
@@ -253,7 +265,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (ok) ok = score_s(0);
       if (ok) ok = score_p(0);
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int st = j & 1;
+        const int st = j % RING;
         if (j + 1 < n_tiles && !score_s(j + 1)) { ok = false; break; }
         const uint32_t k_addr = smem_u32(sK + st * TILE_BYTES);
         // 16 keys per step; the packed columns of the 32 keys [32 g, 32 g + 32) start at column
@@ -285,26 +297,36 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int my_row = quarter * 32 + lane;
     const bool row_ok = my_row < rows;
     const int64_t stat_index = int64_t(head) * p.total_q + q_row + my_row;
-    // delta of the row: the two halves of its elements, joined through shared memory
-    float part = 0.f;
-    if (row_ok) {
-      const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row + my_row) * p.hq + head) * p.dim;
-      const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row + my_row) * p.grad_row + head * p.grad_head;
-#pragma unroll 4
-      for (int e = half * (DP / 2); e < (half + 1) * (DP / 2); e += 8) {
-        if (e >= p.dim) break;
-        const uint4 a = *reinterpret_cast<const uint4*>(o + e), b = *reinterpret_cast<const uint4*>(g + e);
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    // delta of 16 rows a warp, four elements a lane, whole rows an instruction (one row a thread took 7000
+    // cycles); all loads are on their way before the first sum
+    {
+      const int row0 = warp * 16, e = lane * 4;
+      const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row + row0) * p.hq + head) * p.dim + e;
+      const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row + row0) * p.grad_row + head * p.grad_head + e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = unpack16<FP16>(aw[i]), y = unpack16<FP16>(bw[i]);
-          part = fmaf(x.x, y.x, fmaf(x.y, y.y, part));
+      for (int half16 = 0; half16 < 2; ++half16) {
+        uint2 a[8], b[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          a[r] = b[r] = make_uint2(0, 0);
+          if (row0 + half16 * 8 + r < rows && e < p.dim) {
+            a[r] = *reinterpret_cast<const uint2*>(o + int64_t(half16 * 8 + r) * p.hq * p.dim);
+            b[r] = *reinterpret_cast<const uint2*>(g + (half16 * 8 + r) * p.grad_row);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float2 x0 = unpack16<FP16>(a[r].x), x1 = unpack16<FP16>(a[r].y);
+          const float2 y0 = unpack16<FP16>(b[r].x), y1 = unpack16<FP16>(b[r].y);
+          float sum = fmaf(x0.x, y0.x, fmaf(x0.y, y0.y, fmaf(x1.x, y1.x, x1.y * y1.y)));
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if (lane == r) deltas[row0 + half16 * 8 + r] = sum;
         }
       }
     }
-    halves[half * ROWS + my_row] = part;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = halves[my_row] + halves[ROWS + my_row];
+    const float delta = deltas[my_row];
     if (row_ok && half == 0) p.delta[stat_index] = delta;
     const float lse2 = row_ok ? p.lse[stat_index] * LOG2E : 0.f;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
@@ -326,16 +348,20 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         uint32_t sv[32];
         tmem_ld_32x32(tmem_base + lane_base + C_S + buf * 128 + half * 64 + c * 32, sv);
         tmem_ld_wait();
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 x = ffma2(make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sc2, nl2);
-          float2 e = make_float2(exp2f(x.x), exp2f(x.y));
-          if (!plain) {
-            const int col = half * 64 + c * 32 + 2 * i;
-            if (col >= valid) e.x = 0.f;
-            if (col + 1 >= valid) e.y = 0.f;
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = ffma2(make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sc2, nl2);
+            prob[c * 16 + i] = i % 4 == 3 ? exp2_pair<true>(x) : exp2_pair<false>(x);
           }
-          prob[c * 16 + i] = e;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = ffma2(make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sc2, nl2);
+            const float2 e = exp2_pair<false>(x);
+            const int col = half * 64 + c * 32 + 2 * i;
+            prob[c * 16 + i] = make_float2(col >= valid ? 0.f : e.x, col + 1 >= valid ? 0.f : e.y);
+          }
         }
       }
       if (!mbar_wait(dp_full, j & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
@@ -362,9 +388,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (ok) ok = mbar_wait(dq_done, 0, guard, kTimeoutEpilogue);
     if (n_tiles == 0 || ok) {
       tc_fence_after_sync();
-      uint16_t* dst = static_cast<uint16_t*>(p.dq) + (int64_t(q_row + my_row) * p.hq + head) * p.dim;
-      store_rows<DP, FP16>(dst, tmem_base + lane_base + C_DQ, p.dim, p.scale, row_ok, n_tiles > 0, true,
-                           half * (DP / 64), (half + 1) * (DP / 64));
+      // every product is complete: the stages lie over the Q and dO tiles
+      if (half < DP / 64) {
+        const int64_t row = int64_t(q_row) + quarter * 32;
+        store_columns<FP16>(static_cast<uint16_t*>(p.dq) + (row * p.hq + head) * p.dim + half * 64, int64_t(p.hq) * p.dim,
+                            tmem_base + lane_base + C_DQ + half * 64, p.dim - half * 64, p.scale,
+                            rows - quarter * 32, n_tiles > 0, true, smem_u32(smem + warp * 4096), lane);
+      }
     }
     if (span.unit_in_sequence == -2) {  // rows behind the last sequence
       const int words = p.dim / 8;
@@ -397,25 +427,27 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                    const BwdParams p) {
   constexpr int ATOMS = DP / 64;
   constexpr int TILE_BYTES = ATOMS * HALF_BYTES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // the swizzle counts addresses in blocks of 1024 bytes
   uint8_t* sK = smem;
   uint8_t* sV = smem + TILE_BYTES;
-  uint8_t* sQ = smem + 2 * TILE_BYTES;      // [2]
-  uint8_t* sdO = smem + 4 * TILE_BYTES;     // [2]
-  float* stats = reinterpret_cast<float*>(smem + 6 * TILE_BYTES);  // [2][-lse log2(e) [128], -delta [128]]
+  uint8_t* sQ = smem + 2 * TILE_BYTES;      // [RING]
+  uint8_t* sdO = smem + 5 * TILE_BYTES;     // [2]
+  float* stats = reinterpret_cast<float*>(smem + 7 * TILE_BYTES);  // [2][-lse log2(e) [128], -delta [128]]
   uint64_t* bars = reinterpret_cast<uint64_t*>(stats + 4 * ROWS);
   uint64_t* kv_full = bars;
-  uint64_t* qd_full = bars + 1;     // [2]
-  uint64_t* qd_empty = bars + 3;    // [2]
-  uint64_t* st_full = bars + 5;     // S^T of an item complete
-  uint64_t* dp_full = bars + 6;     // dP^T of an item complete
-  uint64_t* pt_ready = bars + 7;    // [2] P^T of query chunk c of both halves written (count 8)
-  uint64_t* ds_ready = bars + 9;    // dS^T written (count 8)
-  uint64_t* grad_done = bars + 10;  // all gradient products finished
-  uint64_t* stats_bar = bars + 11;  // lse and delta of an item staged (count 256)
-  uint64_t* qd_clean = bars + 12;   // [2] rows of a ragged query block behind the last query cleared
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint64_t* q_full = bars + 1;      // [RING]
+  uint64_t* q_empty = bars + 4;     // [RING]
+  uint64_t* do_full = bars + 7;     // [2]
+  uint64_t* do_empty = bars + 9;    // [2]
+  uint64_t* st_full = bars + 11;    // S^T of an item complete
+  uint64_t* dp_full = bars + 12;    // dP^T of an item complete
+  uint64_t* pt_ready = bars + 13;   // [2] P^T of query chunk c of both halves written (count 8)
+  uint64_t* ds_ready = bars + 15;   // dS^T written (count 8)
+  uint64_t* grad_done = bars + 16;  // all gradient products finished
+  uint64_t* stats_full = bars + 17; // [2] lse and delta of an item staged
+  uint64_t* stats_empty = bars + 19;  // [2] and read (count 8)
+  uint64_t* clean = bars + 21;      // [2] rows of a ragged query block behind the last query cleared
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
 
@@ -433,16 +465,21 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     *abort_flag = 0;
     mbar_init(kv_full, 1);
     mbar_init(grad_done, 1);
-    mbar_init(stats_bar, 256);
     mbar_init(st_full, 1);
     mbar_init(dp_full, 1);
     mbar_init(&pt_ready[0], 8);
     mbar_init(&pt_ready[1], 8);
     mbar_init(ds_ready, 8);
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&qd_clean[i], 1);
-      mbar_init(&qd_full[i], 1);
-      mbar_init(&qd_empty[i], 1);
+      mbar_init(&do_full[i], 1);
+      mbar_init(&do_empty[i], 1);
+      mbar_init(&clean[i], 1);
+      mbar_init(&stats_full[i], 1);
+      mbar_init(&stats_empty[i], 8);
     }
     mbar_fence_init();
   }
@@ -478,27 +515,52 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       bool ok = true;
       int head = kv_head * p.group, block = 0;
       for (int i = 0; i < n_items && ok; ++i) {
-        const int st = i & 1;
-        ok = mbar_wait_w(&qd_empty[st], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer);
+        const int st = i % RING, sd = i & 1;
+        ok = mbar_wait_w(&q_empty[st], ((i / RING) & 1) ^ 1, guard, kTimeoutProducer);
         if (!ok) break;
         if (lane == 0) {
-          mbar_expect_tx(&qd_full[st], 2 * TILE_BYTES);
-          load_tile<ATOMS>(sQ + st * TILE_BYTES, &tm_q, &qd_full[st], head, span.q0 + i0 + block * ROWS);
-          load_tile<ATOMS>(sdO + st * TILE_BYTES, &tm_do, &qd_full[st], head, span.q0 + i0 + block * ROWS);
+          mbar_expect_tx(&q_full[st], TILE_BYTES);
+          load_tile<ATOMS>(sQ + st * TILE_BYTES, &tm_q, &q_full[st], head, span.q0 + i0 + block * ROWS);
+        }
+        ok = mbar_wait_w(&do_empty[sd], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(&do_full[sd], TILE_BYTES);
+          load_tile<ATOMS>(sdO + sd * TILE_BYTES, &tm_do, &do_full[sd], head, span.q0 + i0 + block * ROWS);
+        }
+        // -lse * log2(e) (or -inf: probability 0) and -delta of the item's queries
+        {
+          float nl[4], nd[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int q = i0 + block * ROWS + k * 32 + lane;
+            const bool there = q < span.rows;
+            const int64_t at = int64_t(head) * p.total_q + span.q0 + q;
+            nl[k] = there ? -p.lse[at] * LOG2E : -INFINITY;
+            nd[k] = there ? -p.delta[at] : 0.f;
+          }
+          ok = mbar_wait_w(&stats_empty[sd], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer);
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            stats[sd * 2 * ROWS + k * 32 + lane] = nl[k];
+            stats[sd * 2 * ROWS + ROWS + k * 32 + lane] = nd[k];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&stats_full[sd]);
         }
         if (++block == blocks) {
           block = 0;
           ++head;
-          // Nothing is lost by waiting here: the stage of item i + 1 comes free with dK(i - 1), which
-          // is issued behind S^T(i).
           if (ragged) {
-            ok = mbar_wait_w(&qd_full[st], (i >> 1) & 1, guard, kTimeoutProducer);
+            ok = mbar_wait_w(&q_full[st], (i / RING) & 1, guard, kTimeoutProducer) &&
+                 mbar_wait_w(&do_full[sd], (i >> 1) & 1, guard, kTimeoutProducer);
             if (!ok) break;
             clear_rows<ATOMS>(smem_u32(sQ + st * TILE_BYTES), tail_rows, lane);
-            clear_rows<ATOMS>(smem_u32(sdO + st * TILE_BYTES), tail_rows, lane);
+            clear_rows<ATOMS>(smem_u32(sdO + sd * TILE_BYTES), tail_rows, lane);
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&qd_clean[st]);
+            if (lane == 0) mbar_arrive(&clean[sd]);
           }
         }
       }
@@ -517,13 +579,13 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       // S^T of item i (needs its Q in shared memory; the buffer's last reader, dV(i-1), was
       // issued before).
       auto score_s = [&](int i) -> bool {
-        const int st = i & 1;
-        if (!mbar_wait(&qd_full[st], (i >> 1) & 1, guard, kTimeoutMma)) return false;
+        const int st = i % RING, sd = i & 1;
+        if (!mbar_wait(&q_full[st], (i / RING) & 1, guard, kTimeoutMma)) return false;
         if (++block == blocks) {
           block = 0;
           if (ragged) {
-            if (!mbar_wait(&qd_clean[st], (cleaned >> st) & 1, guard, kTimeoutMma)) return false;
-            cleaned ^= 1u << st;
+            if (!mbar_wait(&clean[sd], (cleaned >> sd) & 1, guard, kTimeoutMma)) return false;
+            cleaned ^= 1u << sd;
           }
         }
         tc_fence_after_sync();
@@ -537,8 +599,10 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tc_commit(st_full);
         return true;
       };
-      // dP^T of item i (its dO arrived with Q; the buffer's last reader, dK(i-1), was issued before).
-      auto score_p = [&](int i) {
+      // dP^T of item i (the buffer's last reader, dK(i-1), was issued before).
+      auto score_p = [&](int i) -> bool {
+        if (!mbar_wait(&do_full[i & 1], (i >> 1) & 1, guard, kTimeoutMma)) return false;
+        tc_fence_after_sync();
         const uint32_t do_addr = smem_u32(sdO + (i & 1) * TILE_BYTES);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
@@ -547,14 +611,15 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                       make_smem_desc(do_addr + off, 16, 1024), idesc_s, kk != 0);
         }
         tc_commit(dp_full);
+        return true;
       };
       bool ok = mbar_wait(kv_full, 0, guard, kTimeoutMma);
       if (ok) ok = score_s(0);
-      if (ok) score_p(0);
+      if (ok) ok = score_p(0);
       for (int i = 0; i < n_items && ok; ++i) {
-        const int st = i & 1;
+        const int st = i % RING;
         const uint32_t q_addr = smem_u32(sQ + st * TILE_BYTES);
-        const uint32_t do_addr = smem_u32(sdO + st * TILE_BYTES);
+        const uint32_t do_addr = smem_u32(sdO + (i & 1) * TILE_BYTES);
         // 16 queries per step; the packed columns of the 32 queries [32 g, 32 g + 32) start at
         // column 32 g.  The warps announce P^T in two parts (their first and their second 32
         // columns: g = c and g = 2 + c).
@@ -570,6 +635,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           }
         }
         if (!ok) break;
+        tc_commit(&do_empty[i & 1]);
         if (i + 1 < n_items && !score_s(i + 1)) { ok = false; break; }
         if (!mbar_wait(ds_ready, i & 1, guard, kTimeoutMma)) { ok = false; break; }
         tc_fence_after_sync();
@@ -577,8 +643,8 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         for (int kk = 0; kk < ROWS / 16; ++kk)
           tc_mma_ts(tmem_base + C_DK, tmem_base + C_DPT + (kk >> 1) * 32 + (kk & 1) * 8,
                       make_smem_desc(q_addr + kk * 2048, HALF_BYTES, 1024), idesc_g, (i | kk) != 0);
-        tc_commit(&qd_empty[st]);
-        if (i + 1 < n_items) score_p(i + 1);
+        tc_commit(&q_empty[st]);
+        if (i + 1 < n_items && !score_p(i + 1)) { ok = false; break; }
       }
       if (ok) tc_commit(grad_done);
     }
@@ -589,36 +655,19 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int tid = (warp << 5) + lane;      // 0..255
     const int key = quarter * 32 + lane;     // key row of this thread
     bool ok = n_items > 0;
-    // Per query column the warps need -lse*log2(e) and -delta.  They are staged in shared memory one
-    // item ahead: the global loads of item i + 1 are issued before the work on item i and stored
-    // behind it, so their latency never sits between two items.
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    auto fetch_stat = [&](int g, int block) -> float {
-      // threads 0..127: -lse*log2(e) (or -inf: probability 0), threads 128..255: -delta
-      const int col = i0 + block * ROWS + (tid & (ROWS - 1));
-      const bool valid = col < span.rows;
-      const int64_t at = int64_t(kv_head * p.group + g) * p.total_q + span.q0 + col;
-      if (tid < ROWS) return valid ? -p.lse[at] * LOG2E : -INFINITY;
-      return valid ? -p.delta[at] : 0.f;
-    };
-    if (ok) {
-      stats[tid] = fetch_stat(0, 0);
-      mbar_arrive(stats_bar);
-    }
-    int g = 0, block = 0;
+    int block = 0;
     for (int i = 0; i < n_items && ok; ++i) {
-      const bool more = i + 1 < n_items;
+      const int st = i & 1;
       const int q_first = i0 + block * ROWS;
       const int q_rows = min(ROWS, span.rows - q_first);
-      if (++block == blocks) { block = 0; ++g; }
-      float next_stat = 0.f;
-      if (more) next_stat = fetch_stat(g, block);
-      const float* my_stats = stats + (i & 1) * 2 * ROWS + half * 64;
+      if (++block == blocks) block = 0;
+      const uint32_t my_stats = smem_u32(stats + st * 2 * ROWS + half * 64);
       // query column c sees this key where c >= from, of the block's q_rows; only blocks that mask
       // pay for it, and the test is uniform over the CTA
       const int from = key < k_valid ? k_first + key - shift - q_first : ROWS;
       const bool plain = k_valid == ROWS && q_rows == ROWS && k_first + ROWS - 1 - shift <= q_first;
-      if (!mbar_wait(stats_bar, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
+      if (!mbar_wait(&stats_full[st], (i >> 1) & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
       if (!mbar_wait(st_full, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
       tc_fence_after_sync();
       float2 prob[32];  // the probabilities of this thread's 64 query columns, kept for dS^T
@@ -627,28 +676,35 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         uint32_t sv[32], pp[16];
         tmem_ld_32x32(tmem_base + lane_base + C_ST + half * 64 + c * 32, sv);
         tmem_ld_wait();
-        const float4* nl4 = reinterpret_cast<const float4*>(my_stats + c * 32);
-#pragma unroll
-        for (int k4 = 0; k4 < 8; ++k4) {  // four query columns per step
-          const float4 nl = nl4[k4];
+        auto four = [&](int k4, auto fma) {  // four query columns
+          const uint4 nl = get16(my_stats + c * 128 + k4 * 16);
           const float2 x0 = ffma2(make_float2(__uint_as_float(sv[4 * k4]), __uint_as_float(sv[4 * k4 + 1])), sc2,
-                                  make_float2(nl.x, nl.y));
+                                  make_float2(__uint_as_float(nl.x), __uint_as_float(nl.y)));
           const float2 x1 = ffma2(make_float2(__uint_as_float(sv[4 * k4 + 2]), __uint_as_float(sv[4 * k4 + 3])), sc2,
-                                  make_float2(nl.z, nl.w));
-          float2 e0 = make_float2(exp2f(x0.x), exp2f(x0.y));
-          float2 e1 = make_float2(exp2f(x1.x), exp2f(x1.y));
-          if (!plain) {
+                                  make_float2(__uint_as_float(nl.z), __uint_as_float(nl.w)));
+          prob[c * 16 + 2 * k4] = exp2_pair<false>(x0);
+          prob[c * 16 + 2 * k4 + 1] = exp2_pair<decltype(fma)::value>(x1);
+        };
+        if (plain) {
+#pragma unroll
+          for (int k4 = 0; k4 < 8; ++k4) {
+            if (k4 & 1) four(k4, std::true_type{});
+            else four(k4, std::false_type{});
+          }
+        } else {
+#pragma unroll
+          for (int k4 = 0; k4 < 8; ++k4) {
+            four(k4, std::false_type{});
+            float2 &e0 = prob[c * 16 + 2 * k4], &e1 = prob[c * 16 + 2 * k4 + 1];
             const int col = half * 64 + c * 32 + 4 * k4;
             if (col < from || col >= q_rows) e0.x = 0.f;
             if (col + 1 < from || col + 1 >= q_rows) e0.y = 0.f;
             if (col + 2 < from || col + 2 >= q_rows) e1.x = 0.f;
             if (col + 3 < from || col + 3 >= q_rows) e1.y = 0.f;
           }
-          prob[c * 16 + 2 * k4] = e0;
-          prob[c * 16 + 2 * k4 + 1] = e1;
-          pp[2 * k4] = pack16<FP16>(e0.x, e0.y);
-          pp[2 * k4 + 1] = pack16<FP16>(e1.x, e1.y);
         }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) pp[k] = pack16<FP16>(prob[c * 16 + k].x, prob[c * 16 + k].y);
         // the packed results land in columns this thread has already read
         tmem_st_32x16(tmem_base + lane_base + C_ST + half * 64 + c * 32, pp);
         tmem_st_wait();
@@ -663,14 +719,13 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         uint32_t dv[32], dd[16];
         tmem_ld_32x32(tmem_base + lane_base + C_DPT + half * 64 + c * 32, dv);
         tmem_ld_wait();
-        const float4* nd4 = reinterpret_cast<const float4*>(my_stats + ROWS + c * 32);
 #pragma unroll
         for (int k4 = 0; k4 < 8; ++k4) {
-          const float4 nd = nd4[k4];
+          const uint4 nd = get16(my_stats + ROWS * 4 + c * 128 + k4 * 16);
           const float2 g0 = fadd2(make_float2(__uint_as_float(dv[4 * k4]), __uint_as_float(dv[4 * k4 + 1])),
-                                  make_float2(nd.x, nd.y));
+                                  make_float2(__uint_as_float(nd.x), __uint_as_float(nd.y)));
           const float2 g1 = fadd2(make_float2(__uint_as_float(dv[4 * k4 + 2]), __uint_as_float(dv[4 * k4 + 3])),
-                                  make_float2(nd.z, nd.w));
+                                  make_float2(__uint_as_float(nd.z), __uint_as_float(nd.w)));
           const float2 d0 = fmul2(prob[c * 16 + 2 * k4], g0), d1 = fmul2(prob[c * 16 + 2 * k4 + 1], g1);
           dd[2 * k4] = pack16<FP16>(d0.x, d0.y);
           dd[2 * k4 + 1] = pack16<FP16>(d1.x, d1.y);
@@ -680,23 +735,24 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
-      // The other stats buffer was last read for item i - 1; every thread has passed the wait
-      // of phase i above, which all threads entered only after finishing item i - 1.
-      if (more) {
-        stats[((i + 1) & 1) * 2 * ROWS + tid] = next_stat;
-        mbar_arrive(stats_bar);
+      if (lane == 0) {
+        mbar_arrive(ds_ready);
+        mbar_arrive(&stats_empty[st]);
       }
     }
     if (ok) ok = mbar_wait(grad_done, 0, guard, kTimeoutEpilogue);
     if (n_items == 0 || ok) {
       tc_fence_after_sync();
-      // the two halves write one gradient each
-      uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) +
-                      (int64_t(span.k0 + k_first + key) * p.hkv + kv_head) * p.dim;
-      // rows that are no keys (the room behind them) get zeros
-      store_rows<DP, FP16>(dst, tmem_base + lane_base + (half == 0 ? C_DV : C_DK), p.dim, half == 0 ? 1.f : p.scale,
-                           key < k_rows, n_items > 0, key < k_valid, 0, DP / 32);
+      // the two halves write one gradient each; every product is complete: the stages lie over the K
+      // and V tiles.  Rows that are no keys (the room behind them) get zeros.
+      const int64_t row = int64_t(span.k0) + k_first + quarter * 32;
+      uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) + (row * p.hkv + kv_head) * p.dim;
+#pragma unroll 1
+      for (int c = 0; c < DP / 64; ++c)
+        store_columns<FP16>(dst + c * 64, int64_t(p.hkv) * p.dim,
+                            tmem_base + lane_base + (half == 0 ? C_DV : C_DK) + c * 64, p.dim - c * 64,
+                            half == 0 ? 1.f : p.scale, k_rows - quarter * 32, n_items > 0, key < k_valid,
+                            smem_u32(smem + warp * 4096), lane);
     }
     if (span.unit_in_sequence == -2) {  // rows behind the last sequence
       const int words = p.dim / 8;

@@ -28,6 +28,32 @@ __device__ __forceinline__ void store16(void* to, uint4 v) {
   asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};"
                ::"l"(__cvta_generic_to_global(to)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+// 32 rows x 128 bytes of a warp from its stage in shared memory (4 KB; 16-byte word w of row r lies at word
+// w ^ (r & 7)) to global rows `pitch` bytes apart: the first `live` rows, of which `bytes` are left from
+// `dst` on.  Whole rows an instruction; stores of one row a thread would touch 32 lines each.
+__device__ __forceinline__ uint32_t stage_word(uint32_t stage, int row, int word) {
+  return stage + row * 128 + ((word ^ row) & 7) * 16;
+}
+__device__ __forceinline__ void flush_rows(uint32_t stage, uint8_t* dst, int64_t pitch, int bytes, int live, int lane) {
+  __syncwarp();
+  const int w = lane & 7, first = lane >> 3;
+  uint4 v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = get16(stage_word(stage, k * 4 + first, w));
+  if (w * 16 < bytes) {
+    uint8_t* to = dst + first * pitch + w * 16;
+    if (live >= 32) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k, to += 4 * pitch) store16(to, v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k, to += 4 * pitch)
+        if (k * 4 + first < live) store16(to, v[k]);
+    }
+  }
+  __syncwarp();
+}
+
 // Clears rows [from, 128) of a tile (ATOMS blocks of 128 rows x 128 bytes; a row is 128 bytes of each
 // block whatever the swizzle, which permutes within the row); converged warp.
 template <int ATOMS>
