@@ -237,11 +237,12 @@ bool few_rows(const agb::PackedArgs& a) {
   return a.total_q * heads <= int64_t(16) * a.sequences;
 }
 
-// Keys of a chunk: about three CTAs for every place (two on an SM), and never so few that joining them shows.
+// Keys of a chunk: about three for every warp that the GPU holds (eight an SM), and not so few that
+// starting and joining them shows.
 int rows_chunk(const agb::PackedArgs& a, int sms) {
   const int64_t work = a.total_k * a.hkv * agb::packed_rows_pieces(a.hq / a.hkv);
-  const int64_t chunk = (work / (int64_t(sms) * 2 * 3) + 63) / 64 * 64;
-  return int(std::min<int64_t>(std::max<int64_t>(chunk, 256), 8192));
+  const int64_t chunk = (work / (int64_t(sms) * 8 * 3) + 63) / 64 * 64;
+  return int(std::min<int64_t>(std::max<int64_t>(chunk, 128), 8192));
 }
 
 // Key ranges of a tile: the count that makes the estimated launch shortest.  In units of one key
@@ -289,7 +290,7 @@ std::pair<Tensor, Tensor> attend(const Tensor& query, const Tensor& key, const T
     const int64_t pieces = agb::packed_rows_pieces(group);
     a.chunk = rows_chunk(a, sms);
     if (a.total_k > a.chunk) {
-      const int64_t slots = (a.total_k / a.chunk + a.sequences) * a.hkv * pieces * 16;
+      const int64_t slots = (a.total_k / a.chunk + 3 * int64_t(a.sequences)) * a.hkv * pieces * 16;
       part_out = empty_fp32({slots, a.dim}, q);
       part_lse = empty_fp32({slots}, q);
       a.part_out = part_out.data_ptr<float>();

@@ -46,6 +46,7 @@ struct BwdParams {
   float* delta;         // [hq, total_q]
   void* dq; void* dk; void* dv;  // dense
   int hq, hkv, group, dim;
+  int share;            // CTAs (a cluster) that share the query heads of a key tile
   float scale, scale_log2;
   int* status;
 };
@@ -303,26 +304,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const int row0 = warp * 16, e = lane * 4;
       const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row + row0) * p.hq + head) * p.dim + e;
       const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row + row0) * p.grad_row + head * p.grad_head + e;
+      uint2 a[16], b[16];
 #pragma unroll
-      for (int half16 = 0; half16 < 2; ++half16) {
-        uint2 a[8], b[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          a[r] = b[r] = make_uint2(0, 0);
-          if (row0 + half16 * 8 + r < rows && e < p.dim) {
-            a[r] = *reinterpret_cast<const uint2*>(o + int64_t(half16 * 8 + r) * p.hq * p.dim);
-            b[r] = *reinterpret_cast<const uint2*>(g + (half16 * 8 + r) * p.grad_row);
-          }
+      for (int r = 0; r < 16; ++r) {
+        a[r] = b[r] = make_uint2(0, 0);
+        if (row0 + r < rows && e < p.dim) {
+          a[r] = *reinterpret_cast<const uint2*>(o + int64_t(r) * p.hq * p.dim);
+          b[r] = *reinterpret_cast<const uint2*>(g + r * p.grad_row);
         }
+      }
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float2 x0 = unpack16<FP16>(a[r].x), x1 = unpack16<FP16>(a[r].y);
-          const float2 y0 = unpack16<FP16>(b[r].x), y1 = unpack16<FP16>(b[r].y);
-          float sum = fmaf(x0.x, y0.x, fmaf(x0.y, y0.y, fmaf(x1.x, y1.x, x1.y * y1.y)));
+      for (int r = 0; r < 16; ++r) {
+        const float2 x0 = unpack16<FP16>(a[r].x), x1 = unpack16<FP16>(a[r].y);
+        const float2 y0 = unpack16<FP16>(b[r].x), y1 = unpack16<FP16>(b[r].y);
+        float sum = fmaf(x0.x, y0.x, fmaf(x0.y, y0.y, fmaf(x1.x, y1.x, x1.y * y1.y)));
 #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          if (lane == r) deltas[row0 + half16 * 8 + r] = sum;
-        }
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == r) deltas[row0 + r] = sum;
       }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -413,6 +411,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------- dK / dV
+// With few key tiles, up to four CTAs of a cluster take a part of the group's query heads each and add
+// their accumulators at the end through each other's shared memory, in the order of their ranks: the
+// first key tile of a sequence is seen by all of its queries and would decide how long the launch takes.
 // Items are (query head of the group, block of 128 query rows that can see the tile), issued
 // dV(i) | S^T(i+1) | dK(i) | dP^T(i+1): the exponentials of item i+1 run under dK(i) and dP^T(i+1), its
 // dS^T under dV(i+1) and S^T(i+2).  Single score buffers: refilling one behind the product that
@@ -452,13 +453,15 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kv_head = int(blockIdx.x % unsigned(p.hkv));
-  const int unit = int(blockIdx.x / unsigned(p.hkv));
+  const int member = int(blockIdx.x % unsigned(p.share));  // rank in the cluster
+  const int kv_head = int((blockIdx.x / unsigned(p.share)) % unsigned(p.hkv));
+  const int unit = int(blockIdx.x / (unsigned(p.share) * unsigned(p.hkv)));
+  const int my_heads = p.group / p.share, head0 = kv_head * p.group + member * my_heads;
   const WaitGuard guard{abort_flag, p.status};
 
   if (warp == 0) {
     const PackedSpan span = find_piece(unit, ROWS, true, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
-                                       p.total_q, p.total_k, kv_head == 0 ? p.status : nullptr);
+                                       p.total_q, p.total_k, kv_head == 0 && member == 0 ? p.status : nullptr);
     if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
   }
   if (warp == 1 && lane == 0) {
@@ -501,7 +504,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int shift = span.keys - span.rows;                                // query i sees the keys up to i + shift
   const int i0 = max(0, k_first - shift);                                 // the first query that sees the tile
   const int blocks = covered && k_valid > 0 && i0 < span.rows ? (span.rows - i0 + ROWS - 1) / ROWS : 0;
-  const int n_items = blocks * p.group;
+  const int n_items = blocks * my_heads;
   const int tail_rows = span.rows - i0 - (blocks - 1) * ROWS;             // queries of the last block
   const bool ragged = blocks > 0 && tail_rows < ROWS;
 
@@ -513,7 +516,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         load_tile<ATOMS>(sV, &tm_v, kv_full, kv_head, span.k0 + k_first);
       }
       bool ok = true;
-      int head = kv_head * p.group, block = 0;
+      int head = head0, block = 0;
       for (int i = 0; i < n_items && ok; ++i) {
         const int st = i % RING, sd = i & 1;
         ok = mbar_wait_w(&q_empty[st], ((i / RING) & 1) ^ 1, guard, kTimeoutProducer);
@@ -741,7 +744,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
     if (ok) ok = mbar_wait(grad_done, 0, guard, kTimeoutEpilogue);
-    if (n_items == 0 || ok) {
+    if ((n_items == 0 && member == 0) || (ok && p.share == 1)) {
       tc_fence_after_sync();
       // the two halves write one gradient each; every product is complete: the stages lie over the K
       // and V tiles.  Rows that are no keys (the room behind them) get zeros.
@@ -754,12 +757,82 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                             half == 0 ? 1.f : p.scale, k_rows - quarter * 32, n_items > 0, key < k_valid,
                             smem_u32(smem + warp * 4096), lane);
     }
-    if (span.unit_in_sequence == -2) {  // rows behind the last sequence
+    if (span.unit_in_sequence == -2 && member == 0) {  // rows behind the last sequence
       const int words = p.dim / 8;
       for (int i = tid; i < span.rows * words; i += 256) {
         const int64_t at = ((int64_t(span.k0) + i / words) * p.hkv + kv_head) * p.dim + (i % words) * 8;
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dk) + at) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dv) + at) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  if (p.share > 1 && n_items > 0) {
+    // dV and dK side by side are 2 DP columns; each member adds up `width` of them.
+    const int width = 2 * DP / p.share;
+    const int quarter = warp & 3, half = (warp >> 2) & 1;
+    const int key = quarter * 32 + lane;
+    const uint32_t column0 = tmem_base + (uint32_t(quarter * 32) << 16) + C_DV;
+    auto column = [&](int c) { return c < DP ? c : c - DP + int(C_DK - C_DV); };
+    // 16-byte word w (of a row of `width` FP32 columns) of a sender's part
+    auto place = [&](int sender, int row, int w) {
+      return smem_u32(smem) + ((sender * ROWS + row) * width + (w & ~7) * 4) * 4 + ((w ^ row) & 7) * 16;
+    };
+    tc_fence_before_sync();
+    cluster_sync();  // no member reads its tiles any more
+    tc_fence_after_sync();
+    if (warp < 8) {
+      for (int to = 0; to < p.share; ++to) {
+        if (to == member) continue;
+        const int sender = member < to ? member : member - 1;
+        for (int c = half * 32; c < width; c += 64) {
+          uint32_t o[32];
+          tmem_ld_32x32(column0 + column(to * width + c), o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            put16_member(place(sender, key, c / 4 + g), to, make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]));
+        }
+      }
+    }
+    cluster_sync();
+    if (warp < 8) {
+      for (int c = half * 32; c < width; c += 64) {
+        const int at = member * width + c;
+        uint32_t o[32];
+        tmem_ld_32x32(column0 + column(at), o);
+        tmem_ld_wait();
+        float sum[32];
+#pragma unroll 1
+        for (int from = 0; from < p.share; ++from) {
+          const int sender = from < member ? from : from - 1;
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const uint4 v = from == member ? make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3])
+                                           : get16(place(sender, key, c / 4 + g));
+            sum[4 * g] = __uint_as_float(v.x) + (from == 0 ? 0.f : sum[4 * g]);
+            sum[4 * g + 1] = __uint_as_float(v.y) + (from == 0 ? 0.f : sum[4 * g + 1]);
+            sum[4 * g + 2] = __uint_as_float(v.z) + (from == 0 ? 0.f : sum[4 * g + 2]);
+            sum[4 * g + 3] = __uint_as_float(v.w) + (from == 0 ? 0.f : sum[4 * g + 3]);
+          }
+        }
+        if (key < k_rows) {  // rows that are no keys (the room behind them) get zeros
+          const bool is_dv = at < DP;
+          const int d0 = is_dv ? at : at - DP;
+          const float scale = key < k_valid ? (is_dv ? 1.f : p.scale) : 0.f;
+          uint16_t* dst = static_cast<uint16_t*>(is_dv ? p.dv : p.dk) +
+                          ((int64_t(span.k0) + k_first + key) * p.hkv + kv_head) * p.dim + d0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (key < k_valid) {
+              v.x = pack16<FP16>(sum[8 * g] * scale, sum[8 * g + 1] * scale);
+              v.y = pack16<FP16>(sum[8 * g + 2] * scale, sum[8 * g + 3] * scale);
+              v.z = pack16<FP16>(sum[8 * g + 4] * scale, sum[8 * g + 5] * scale);
+              v.w = pack16<FP16>(sum[8 * g + 6] * scale, sum[8 * g + 7] * scale);
+            }
+            if (d0 + g * 8 < p.dim) store16(dst + g * 8, v);
+          }
+        }
       }
     }
   }
@@ -780,14 +853,26 @@ cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap&
     e = cudaFuncSetAttribute(packed_dkdv_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<DP>());
   if (e != cudaSuccess) return e;
   const int64_t q_grid = (p.total_q / ROWS + p.sequences + 1) * p.hq;
-  const int64_t k_grid = (p.total_k / ROWS + p.sequences + 1) * p.hkv;
+  const int64_t k_units = (p.total_k / ROWS + p.sequences + 1) * p.hkv, k_grid = k_units * p.share;
   if (q_grid > 2147483647ll || k_grid > 2147483647ll) {
     set_error_detail("packed_attention: too many tiles for one launch");
     return cudaErrorInvalidValue;
   }
   packed_dq_kernel<DP, FP16><<<unsigned(q_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
-  packed_dkdv_kernel<DP, FP16><<<unsigned(k_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = unsigned(p.share);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(k_grid));
+  config.blockDim = dim3(BWD_THREADS);
+  config.dynamicSmemBytes = bwd_smem<DP>();
+  config.stream = stream;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, packed_dkdv_kernel<DP, FP16>, tq, tdo, tk, tv, p);
 }
 
 }  // namespace
@@ -809,6 +894,12 @@ cudaError_t packed_attention_bwd(const PackedArgs& a, const PackedGrads& g, cuda
   p.hq = a.hq; p.hkv = a.hkv; p.group = a.hq / a.hkv; p.dim = a.dim;
   p.scale = a.scale; p.scale_log2 = a.scale * LOG2E;
   p.status = a.status;
+  // until there are two CTAs for every SM, as far as the group has heads to share out (more only add starts
+  // and ends: 198 us against 116 with four members where two give 3.5 CTAs an SM)
+  p.share = 1;
+  while (p.share < 4 && p.group % (2 * p.share) == 0 &&
+         (a.total_k / ROWS + a.sequences) * a.hkv * p.share < int64_t(2) * a.sm_count)
+    p.share *= 2;
   if (a.dim <= 64)
     return a.fp16 ? launch<64, true>(p, tq, tdo, tk, tv, stream) : launch<64, false>(p, tq, tdo, tk, tv, stream);
   return a.fp16 ? launch<128, true>(p, tq, tdo, tk, tv, stream) : launch<128, false>(p, tq, tdo, tk, tv, stream);

@@ -2,12 +2,17 @@
 //
 // Bound by memory: every key and value is read once for all query heads of its group, which are the
 // rows of one 16-row product (mma.sync: with 4 to 16 useful rows the 128-row products of the tile
-// kernel would idle, and the tensor core is far from being the limit here).  A CTA of four warps
-// works on a chunk of a sequence's keys for one key head; its warps take tiles of 16 keys in turn,
-// each with its own ring of three stages (cp.async, no barrier between the warps), running maximum
-// and FP32 accumulators.  The four are joined in shared memory, and a sequence of several chunks by
-// a second launch, both in a fixed order.  Keys behind the last one are never read: their rows are
-// filled with zeros.
+// kernel would idle, and the tensor core is far from being the limit here).  Every warp works by itself,
+// with its own ring of three stages of 16 keys (cp.async), running maximum and FP32 accumulators, on
+// jobs of (sequence, 16 rows, chunk of keys, key head); eight warps an SM keep 128 KB on their way, so
+// the start and the end of one warp's job (2 to 3 us) hide behind the others.  (Four warps on one chunk,
+// joined in shared memory, all stood still there: 129 us against NEW_LONG for 131071 keys.)  A
+// sequence of several chunks is joined by a second launch, in a fixed order.  Keys behind the last
+// one are never read: their rows are filled with zeros.
+//
+// Jobs are numbered over the keys that exist, sequence by sequence, and dealt out to as many warps as
+// the GPU holds: a cache has room that nobody uses yet, and a block for every chunk of that room
+// cost as much as half of the real ones.
 #include "agb.h"
 #include "packed.h"
 #include "packed_common.cuh"
@@ -38,6 +43,7 @@ struct RowsParams {
   int hq, hkv, group, dim, pieces, chunk;
   float scale_log2;
   float* part_out; float* part_lse;
+  int sm_count, most_jobs;
   int* status;
 };
 
@@ -72,41 +78,95 @@ __device__ __forceinline__ uint32_t word_at(int row, int word) {
   return uint32_t(row * DP * 2 + ((word & ~7) | ((word ^ row) & 7)) * 16);
 }
 
+// The sequence of a job (by_row 0: number `at`) or of a query row (by_row 1).  A sequence has `blocks`
+// blocks of 16 rows times `chunks` chunks of `length` keys: as many chunks as `p.chunk` asks for, or
+// fewer where it has several blocks, so that the jobs of all stay within total_k / chunk + 3 sequences.
+// Converged warp; 32 sequences a step.  Sequences whose offsets do not fit have no jobs and no rows.
+struct JobSpan {
+  int sequence;  // -1: none
+  int first, chunks, length;
+  int q0, rows, k0, keys;
+};
+__device__ inline JobSpan find_job(int at, bool by_row, int heads, const RowsParams& p, int* status) {
+  const int lane = threadIdx.x & 31;
+  JobSpan span{-1, 0, 0, 0, 0, 0, 0, 0};
+  int before = 0;  // jobs of earlier sequences
+  for (int base = 0; base < p.sequences; base += 32) {
+    const int s = base + lane;
+    const bool there = s < p.sequences;
+    const int q0 = p.q_offsets[there ? s : 0], q1 = p.q_offsets[there ? s + 1 : 0];
+    const int k0 = p.k_offsets[there ? s : 0], k1 = p.k_offsets[there ? s + 1 : 0];
+    const int keys = there && p.k_lengths ? p.k_lengths[s] : k1 - k0;
+    const bool fits = q0 >= 0 && q1 >= q0 && q1 <= p.total_q && k0 >= 0 && k1 >= k0 && k1 <= p.total_k && keys >= 0 &&
+                      keys <= k1 - k0;
+    if (there && status && (!fits || (s == 0 && (q0 != 0 || k0 != 0)))) atomicCAS(status, 0, kBadIndex);
+    int chunks = 0, jobs = 0;
+    if (there && fits && q1 > q0) {
+      const int blocks = ((q1 - q0) * heads + QROWS - 1) / QROWS;
+      const int asked = (keys + p.chunk - 1) / p.chunk;
+      chunks = blocks == 1 ? max(1, asked) : max(1, asked / blocks);
+      jobs = chunks * blocks;
+    }
+    int sum = jobs;  // inclusive over the lanes
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    const bool here = jobs > 0 && (by_row ? at >= q0 && at < q1 : at < before + sum);
+    const unsigned votes = __ballot_sync(0xffffffffu, here);
+    if (votes) {
+      const int owner = __ffs(votes) - 1;
+      auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, owner); };
+      span.sequence = base + owner;
+      span.chunks = of(chunks);
+      span.first = before + of(sum - jobs);
+      span.q0 = of(q0);
+      span.rows = of(q1) - span.q0;
+      span.k0 = of(k0);
+      span.keys = of(keys);
+      span.length = span.chunks == 1 ? span.keys : ((span.keys + span.chunks - 1) / span.chunks + KEYS - 1) / KEYS * KEYS;
+      return span;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return span;
+}
+
 template <int DP, bool FP16>
 __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ PackedSpan span_smem;
-  __shared__ float stat[WARPS][QROWS][2];  // maximum and sum of every warp's rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int piece = int(blockIdx.x % unsigned(p.pieces));
-  const int kv_head = int((blockIdx.x / unsigned(p.pieces)) % unsigned(p.hkv));
-  const int unit = int(blockIdx.x / (unsigned(p.pieces) * unsigned(p.hkv)));
-  if (warp == 0) {
-    const PackedSpan found = find_unit(unit, p.chunk, true, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
-                                       p.total_q, p.total_k, kv_head == 0 && piece == 0 ? p.status : nullptr);
-    if (lane == 0) span_smem = found;
-  }
-  __syncthreads();
-  const PackedSpan span = span_smem;
-  const int head0 = kv_head * p.group + piece * QROWS;
-  const int heads = min(QROWS, p.group - piece * QROWS);  // query heads side by side in the rows
-  if (unit == 0) {  // rows behind the last sequence
-    const int end = min(int64_t(max(p.q_offsets[p.sequences], 0)), p.total_q);
+  const int side = p.hkv * p.pieces;  // jobs side by side
+  if (blockIdx.x < side) {            // rows behind the last sequence
+    const int piece = int(blockIdx.x) % p.pieces, head0 = int(blockIdx.x) / p.pieces * p.group + piece * QROWS;
+    const int heads = min(QROWS, p.group - piece * QROWS);
+    const int end = int(min(int64_t(max(p.q_offsets[p.sequences], 0)), p.total_q));
     const int words = heads * p.dim / 8;
     for (int64_t i = threadIdx.x; i < (p.total_q - end) * words; i += WARPS * 32) {
       const int64_t at = ((end + i / words) * p.hq + head0) * p.dim + (i % words) * 8;
       *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = make_uint4(0, 0, 0, 0);
     }
   }
-  if (span.unit_in_sequence < 0 || span.rows == 0) return;
-  const int flat = span.rows * heads;  // rows of the product, query row by query row
-  const int chunks = (span.keys + p.chunk - 1) / p.chunk;
-  // More rows than one product has are taken block by block over all keys by the first chunk's CTA.
-  const bool split = chunks > 1 && flat <= QROWS;
-  if (span.unit_in_sequence > 0 && (!split || span.unit_in_sequence >= chunks)) return;
-  const int k_begin = split ? span.unit_in_sequence * p.chunk : 0;
-  const int k_end = split ? min(span.keys, k_begin + p.chunk) : span.keys;
-  const int tiles = (k_end - k_begin + KEYS - 1) / KEYS;
+  // neighbouring warps take the same keys of neighbouring heads
+  for (int64_t job = int64_t(blockIdx.x) * WARPS + warp;; job += int64_t(gridDim.x) * WARPS) {
+  const int unit = divide(int(job), side), rest = int(job) - unit * side;
+  const int kv_head = divide(rest, p.pieces), piece = rest - kv_head * p.pieces;
+  const int head0 = kv_head * p.group + piece * QROWS;
+  const int heads = min(QROWS, p.group - piece * QROWS);  // query heads side by side in the rows
+  // the pieces of a group have the same jobs: those of its first
+  const JobSpan span = find_job(unit, false, min(QROWS, p.group), p, p.status);
+  if (span.sequence < 0) return;
+  if (unit >= p.most_jobs) {  // offsets that fall make sequences overlap: more jobs than partial results
+    if (lane == 0 && p.status) atomicCAS(p.status, 0, kBadIndex);
+    return;
+  }
+  const int flat = span.rows * heads;  // rows of the products, query row by query row
+  const int block = (unit - span.first) / span.chunks * QROWS, number = (unit - span.first) % span.chunks;
+  const bool split = span.chunks > 1;
+  const int k_begin = number * span.length;
+  const int k_end = min(span.keys, k_begin + span.length);
+  const int tiles = max(0, (k_end - k_begin + KEYS - 1) / KEYS);
 
   const uint16_t* kp = static_cast<const uint16_t*>(p.k) + kv_head * p.k_head;
   const uint16_t* vp = static_cast<const uint16_t*>(p.v) + kv_head * p.v_head;
@@ -128,11 +188,10 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
     }
   };
 
-  for (int block = 0; block < flat; block += QROWS) {
-    const int own = (tiles - warp + WARPS - 1) / WARPS;  // tiles warp, warp + 4, ...
+  {
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      if (s < own) load(warp + s * WARPS, s);
+      if (s < tiles) load(s, s);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     // queries as the A operand: rows lane / 4 and + 8, columns 2 (lane % 4) and + 8 of every 16
@@ -161,12 +220,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
       for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 
-    for (int i = 0; i < own; ++i) {
+    for (int i = 0; i < tiles; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();
       {
         const int next = i + STAGES - 1;
-        if (next < own) load(warp + next * WARPS, next % STAGES);
+        if (next < tiles) load(next, next % STAGES);
         asm volatile("cp.async.commit_group;" ::: "memory");
       }
       const uint32_t base = mine + (i % STAGES) * 2 * KEYS * DP * 2;
@@ -178,13 +237,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
         mma16<FP16>(s[0], q[kk], b[0], b[1]);
         mma16<FP16>(s[1], q[kk], b[2], b[3]);
       }
-      const int tile = warp + i * WARPS;
       float high[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int key = tile * KEYS + n * 8 + (lane & 3) * 2 + (c & 1);
+          const int key = i * KEYS + n * 8 + (lane & 3) * 2 + (c & 1);
           s[n][c] = key < visible && key < seen[c >> 1] ? s[n][c] * p.scale_log2 : -INFINITY;
           high[c >> 1] = fmaxf(high[c >> 1], s[n][c]);
         }
@@ -230,123 +288,110 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
       __syncwarp();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    // Join the four warps in shared memory, in warp order.
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    }
-    __syncthreads();  // every warp is done with its ring
-    float* acc = reinterpret_cast<float*>(ring);  // [WARPS][QROWS][DP]
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = (lane >> 2) + 8 * r;
-      if ((lane & 3) == 0) {
-        stat[warp][row][0] = top[r];
-        stat[warp][row][1] = sum[r];
-      }
-#pragma unroll
-      for (int d = 0; d < DP / 8; ++d)
-        *reinterpret_cast<float2*>(acc + (warp * QROWS + row) * DP + d * 8 + (lane & 3) * 2) =
-            make_float2(o[d][2 * r], o[d][2 * r + 1]);
-    }
-    __syncthreads();
-    const int quads = p.dim / 4;
-    for (int at = threadIdx.x; at < min(QROWS, flat - block) * quads; at += WARPS * 32) {
-      const int row = at / quads, e = (at % quads) * 4;
-      float high = -INFINITY, total = 0.f;
-      for (int w = 0; w < WARPS; ++w) high = fmaxf(high, stat[w][row][0]);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < WARPS; ++w) {
-        const float share = stat[w][row][0] == -INFINITY ? 0.f : exp2f(stat[w][row][0] - high);
-        const float4 y = *reinterpret_cast<const float4*>(acc + (w * QROWS + row) * DP + e);
-        total += share * stat[w][row][1];
-        x.x += share * y.x; x.y += share * y.y; x.z += share * y.z; x.w += share * y.w;
-      }
-      const float inv = total == 0.f ? 0.f : 1.f / total;
-      x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
-      const int f = block + row;
+      const int f = block + (lane >> 2) + 8 * r;
+      if (f >= flat) continue;
+      const float inv = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+      const float log_sum = sum[r] == 0.f ? -INFINITY : top[r] + log2f(sum[r]);
       if (split) {
-        const int64_t slot = ((int64_t(unit) * p.hkv + kv_head) * p.pieces + piece) * QROWS + f;
-        *reinterpret_cast<float4*>(p.part_out + slot * p.dim + e) = x;
-        if (e == 0) p.part_lse[slot] = total == 0.f ? -INFINITY : high + log2f(total);
+        const int64_t slot = ((int64_t(unit) * p.hkv + kv_head) * p.pieces + piece) * QROWS + f - block;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          const int e = d * 8 + (lane & 3) * 2;
+          if (e < p.dim)
+            *reinterpret_cast<float2*>(p.part_out + slot * p.dim + e) = make_float2(o[d][2 * r] * inv, o[d][2 * r + 1] * inv);
+        }
+        if ((lane & 3) == 0) p.part_lse[slot] = log_sum;
       } else {
         const int64_t q_row = int64_t(span.q0) + f / heads;
         const int head = head0 + f % heads;
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (q_row * p.hq + head) * p.dim + e) =
-            make_uint2(pack16<FP16>(x.x, x.y), pack16<FP16>(x.z, x.w));
-        if (e == 0 && p.lse)
-          p.lse[int64_t(head) * p.total_q + q_row] = total == 0.f ? -INFINITY : (high + log2f(total)) * 0.6931471805599453f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (q_row * p.hq + head) * p.dim;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          const int e = d * 8 + (lane & 3) * 2;
+          if (e < p.dim) *reinterpret_cast<uint32_t*>(dst + e) = pack16<FP16>(o[d][2 * r] * inv, o[d][2 * r + 1] * inv);
+        }
+        if ((lane & 3) == 0 && p.lse) p.lse[int64_t(head) * p.total_q + q_row] = log_sum * 0.6931471805599453f;
       }
     }
-    __syncthreads();  // the ring is loaded again for the next block of rows
+    __syncwarp();  // the ring is loaded again for the next job
+  }
   }
 }
 
 // Joins the chunks of every row that had several: out = sum_c w_c o_c.  One CTA per (query row, head);
-// its warps take chunks in turn and are added in warp order.
-constexpr int JOIN_WARPS = 8;
+// its warps take chunks in turn, relative to a maximum of their own, and are added in warp order.  The
+// weights of 32 chunks are evaluated side by side, so that the results' loads wait for nothing.
+constexpr int JOIN_WARPS = 16;
 template <bool FP16>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) packed_rows_join_kernel(const RowsParams p) {
   __shared__ float4 partial[JOIN_WARPS][32];
-  __shared__ float weight[JOIN_WARPS];
+  __shared__ float weight[JOIN_WARPS], tops[JOIN_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int row = int(blockIdx.x / unsigned(p.hq)), head = int(blockIdx.x % unsigned(p.hq));
-  // the sequence of the row: 32-way search for the last s with q_offsets[s] <= row
-  int low = 0, count = p.sequences;
-  bool found = true;
-  while (count > 0) {
-    const int stride = (count + 31) / 32;
-    const bool reached = lane * stride < count && p.q_offsets[low + lane * stride] <= row;
-    const unsigned votes = __ballot_sync(0xffffffffu, reached);
-    if (votes == 0) {
-      found = false;
-      break;
-    }
-    const int last = 31 - __clz(votes);
-    const int behind = count - last * stride;
-    low += last * stride;
-    count = stride == 1 ? 0 : (behind < stride ? behind : stride);
-  }
-  const int q0 = p.q_offsets[low], q1 = p.q_offsets[low + 1];
-  const int k0 = p.k_offsets[low], k1 = p.k_offsets[low + 1];
-  const int keys = p.k_lengths ? p.k_lengths[low] : k1 - k0;
-  found = found && row >= q0 && row < q1 && q1 <= p.total_q && k0 >= 0 && k1 >= k0 && k1 <= p.total_k && keys >= 0 &&
-          keys <= k1 - k0;
+  const JobSpan span = find_job(row, true, min(QROWS, p.group), p, nullptr);
   const int kv_head = head / p.group, in_group = head % p.group;
   const int piece = in_group / QROWS;
   const int heads = min(QROWS, p.group - piece * QROWS);
-  const int chunks = (keys + p.chunk - 1) / p.chunk;
+  const int chunks = span.chunks;
   after_previous_launch();
-  if (!found || chunks <= 1 || (q1 - q0) * heads > QROWS) return;  // written by the first launch
-  const int f = (row - q0) * heads + in_group % QROWS;
+  // written by the first launch, or never (offsets that do not fit)
+  if (span.sequence < 0 || chunks <= 1 || span.first + chunks * ((span.rows * heads + QROWS - 1) / QROWS) > p.most_jobs) return;
+  const int f = (row - span.q0) * heads + in_group % QROWS;
   const int64_t step = int64_t(p.hkv) * p.pieces * QROWS;
-  const int64_t first = ((int64_t(k0) / p.chunk + low) * p.hkv * p.pieces + kv_head * p.pieces + piece) * QROWS + f;
-  float high = -INFINITY;
-  for (int c = lane; c < chunks; c += 32) high = fmaxf(high, p.part_lse[first + c * step]);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+  const int64_t first = ((int64_t(span.first) + f / QROWS * chunks) * p.hkv * p.pieces + kv_head * p.pieces + piece) * QROWS +
+                        f % QROWS;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float total = 0.f;
-#pragma unroll 4
-  for (int c = warp; c < chunks; c += warps) {
-    const int64_t slot = first + c * step;
-    const float l = p.part_lse[slot];
+  float total = 0.f, high = -INFINITY;
+  for (int base = warp; base < chunks; base += 32 * warps) {
+    const int mine = base + lane * warps;
+    const float l = mine < chunks ? p.part_lse[first + mine * step] : -INFINITY;
+    float now = l;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+    now = fmaxf(now, high);
+    const float fade = high == -INFINITY ? 0.f : exp2f(high - now);
+    high = now;
+    x.x *= fade; x.y *= fade; x.z *= fade; x.w *= fade;
+    total *= fade;
     const float share = l == -INFINITY ? 0.f : exp2f(l - high);
-    total += share;
-    if (lane * 4 < p.dim) {
-      const float4 y = *reinterpret_cast<const float4*>(p.part_out + slot * p.dim + lane * 4);
-      x.x += share * y.x; x.y += share * y.y; x.z += share * y.z; x.w += share * y.w;
+    const int count = min(32, (chunks - base + warps - 1) / warps);
+    for (int i = 0; i < count; i += 8) {
+      float4 y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i + k < count && lane * 4 < p.dim)
+          y[k] = *reinterpret_cast<const float4*>(p.part_out + (first + int64_t(base + (i + k) * warps) * step) * p.dim + lane * 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, share, (i + k) & 31);
+        if (i + k < count) {
+          total += w;
+          x.x += w * y[k].x; x.y += w * y[k].y; x.z += w * y[k].z; x.w += w * y[k].w;
+        }
+      }
     }
   }
   partial[warp][lane] = x;
-  if (lane == 0) weight[warp] = total;
+  if (lane == 0) {
+    weight[warp] = total;
+    tops[warp] = high;
+  }
   __syncthreads();
   if (warp != 0) return;
-  for (int w = 1; w < warps; ++w) {
+  for (int w = 0; w < warps; ++w) high = fmaxf(high, tops[w]);
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+  total = 0.f;
+  for (int w = 0; w < warps; ++w) {
+    const float share = tops[w] == -INFINITY ? 0.f : exp2f(tops[w] - high);
     const float4 y = partial[w][lane];
-    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-    total += weight[w];
+    x.x += share * y.x; x.y += share * y.y; x.z += share * y.z; x.w += share * y.w;
+    total += share * weight[w];
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   if (lane * 4 < p.dim)
@@ -361,16 +406,20 @@ cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(packed_rows_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              rows_smem<DP>());
   if (e != cudaSuccess) return e;
-  const int64_t grid = (p.total_k / p.chunk + p.sequences) * p.hkv * p.pieces;
+  const int64_t side = int64_t(p.hkv) * p.pieces, places = int64_t(p.sm_count) * 2;
+  const int64_t jobs = (p.total_k / p.chunk + 3 * int64_t(p.sequences)) * side;  // at most
+  int64_t grid = (jobs + WARPS - 1) / WARPS;
+  if (grid > places) grid = places;
+  if (grid < side) grid = side;  // each of the first `side` CTAs clears rows of one head
   const int64_t joins = p.total_q * p.hq;
-  if (grid > 2147483647ll || joins > 2147483647ll) {
+  if (jobs + grid * WARPS > 2147483647ll || joins > 2147483647ll) {
     set_error_detail("packed_attention: too many chunks for one launch");
     return cudaErrorInvalidValue;
   }
   packed_rows_kernel<DP, FP16><<<unsigned(grid), WARPS * 32, rows_smem<DP>(), stream>>>(p);
   const cudaError_t launched = cudaGetLastError();
   if (launched != cudaSuccess || p.total_k <= p.chunk) return launched;
-  const int64_t most = p.total_k / p.chunk + 1;  // chunks of a sequence
+  const int64_t most = (p.total_k / p.chunk / p.sequences + 4) / 4;  // a quarter of a sequence's chunks
   const int warps = most < JOIN_WARPS ? int(most) : JOIN_WARPS;
   return launch_behind(packed_rows_join_kernel<FP16>, dim3(unsigned(joins)), warps * 32, 0, stream, p);
 }
@@ -390,6 +439,8 @@ cudaError_t packed_attention_rows(const PackedArgs& a, cudaStream_t stream) {
   p.scale_log2 = a.scale * LOG2E;
   p.part_out = a.part_out; p.part_lse = a.part_lse;
   p.status = a.status;
+  p.sm_count = a.sm_count;
+  p.most_jobs = int(a.total_k / a.chunk + 3 * int64_t(a.sequences));
   if (a.dim <= 64) return a.fp16 ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
   return a.fp16 ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
 }

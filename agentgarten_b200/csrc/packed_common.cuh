@@ -28,6 +28,17 @@ __device__ __forceinline__ void store16(void* to, uint4 v) {
   asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};"
                ::"l"(__cvta_generic_to_global(to)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+// The same address of another member of the cluster, and the barrier of all threads of a cluster.
+__device__ __forceinline__ void put16_member(uint32_t address, int member, uint4 v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(member));
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};"
+               ::"r"(remote), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // 32 rows x 128 bytes of a warp from its stage in shared memory (4 KB; 16-byte word w of row r lies at word
 // w ^ (r & 7)) to global rows `pitch` bytes apart: the first `live` rows, of which `bytes` are left from
 // `dst` on.  Whole rows an instruction; stores of one row a thread would touch 32 lines each.

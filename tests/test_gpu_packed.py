@@ -192,6 +192,8 @@ def test_attention_of_single_tokens(k_lengths, heads, kv_heads, dim):
 
 
 def test_attention_of_few_tokens_and_idle_sequences():
+    _check_forward([3, 0, 9, 1, 0, 0, 1, 1, 1, 1, 0, 3], [5000, 7, 3000, 1, 0, 9, 40, 2, 1, 600, 1, 2], 16, 4, 128, BF16, room=3)
+    _check_forward([2, 1, 1, 1], [4000, 900, 30, 1], 40, 1, 64, BF16, room=3)
     _check_forward([0, 1, 3, 0, 2], [40, 900, 33, 7, 2], 8, 2, 128, FP16, room=5, behind=1)
     _check_forward([1] * 30 + [40], [200] * 30 + [300], 8, 2, 128, BF16)
 
@@ -301,6 +303,24 @@ def test_attention_reports_bad_offsets(rows):
         native.ext().status(torch.cuda.current_device()).zero_()
 
 
+def test_attention_reports_offsets_that_fall():
+    """Sequences that overlap because the offsets fall: more work than the rows can have, refused in place."""
+    q, k, v, qo, ko, kl, spans = _case([1] * 40, [700] * 40, 8, 2, 64, BF16)
+    fall = qo.clone()
+    fall[1::2] = 40
+    ops.packed_attention(q, k, v, fall, ko)
+    assert _status() == 7
+    native.ext().status(torch.cuda.current_device()).zero_()
+    fall = ko.clone()
+    fall[1::2] = 28000
+    ops.packed_attention(q, k, v, qo, fall)
+    assert _status() == 7
+    native.ext().status(torch.cuda.current_device()).zero_()
+    out = ops.packed_attention(q, k, v, qo, ko)
+    oracle.assert_close(out, *oracle.attention(q, k, v, spans, 0.125)["out"])
+    assert _status() == 0
+
+
 # ------------------------------------------------------------------------------------ gradients
 def _check_gradients(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw):
     q, k, v, qo, ko, kl, spans = _case(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw)
@@ -339,6 +359,13 @@ def test_gradients_of_head_sizes_and_types(dim, dtype):
                                                   ([50, 140, 10, 4], [20, 100, 0, 3]), ([64, 3], [0, 0]), ([260], [128])])
 def test_gradients_of_continued_prompts(q_lengths, k_lengths):
     _check_gradients(q_lengths, k_lengths, 4, 2, 128, BF16, room=13, behind=2)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 2, 64), (12, 2, 128), (6, 3, 80), (5, 5, 64)])
+@pytest.mark.parametrize("lengths", [[700], [300, 129, 40], [3000, 2900]])
+def test_gradients_with_shared_and_whole_groups(lengths, heads, kv_heads, dim):
+    """Groups whose heads are shared out over four, two or one CTA (the fewer key tiles, the more)."""
+    _check_gradients(lengths, lengths, heads, kv_heads, dim, BF16, behind=3)
 
 
 def test_gradients_repeat_bit_for_bit_and_take_any_layout():
