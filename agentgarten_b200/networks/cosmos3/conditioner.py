@@ -180,6 +180,9 @@ class Cosmos3Conditioner(nn.Module):
         # The text tower's output can be memoised by prompt: prompts repeat across guidance arms
         # and denoising steps of a sampling run.  Off unless a caller switches it on.
         self.cache_text_contexts = False
+        # Prompts of a batch back to back through the text tower, without padded rows.  Off unless a
+        # caller switches it on: its rotary positions are rounded once, not to the tables' type first.
+        self.pack_prompts = False
         self._text_cache: dict[bytes, Any] = {}
 
     def train(self, mode: bool = True) -> "Cosmos3Conditioner":
@@ -249,13 +252,14 @@ class Cosmos3Conditioner(nn.Module):
         return ids, (torch.ones_like(ids, dtype=torch.bool) if valid is None else valid.bool())
 
     def _context(self, ids: torch.Tensor, valid: torch.Tensor):
+        encode = self.text_encoder.encode_packed if self.pack_prompts else self.text_encoder
         if not self.cache_text_contexts:
-            return self.text_encoder(ids, valid)
-        key = (ids * valid).cpu().numpy().tobytes() + valid.cpu().numpy().tobytes()
+            return encode(ids, valid)
+        key = (ids * valid).cpu().numpy().tobytes() + valid.cpu().numpy().tobytes() + bytes((self.pack_prompts,))
         if key not in self._text_cache:
             if len(self._text_cache) > 16:
                 self._text_cache.clear()
-            self._text_cache[key] = self.text_encoder(ids, valid)
+            self._text_cache[key] = encode(ids, valid)
         return self._text_cache[key]
 
     @torch.no_grad()

@@ -269,6 +269,27 @@ class Cosmos3TextLayer(nn.Module):
         return output, key, value
 
 
+    def forward_packed(self, hidden: torch.Tensor, positions: torch.Tensor, frequencies: ops.RotaryFrequencies,
+                       offsets: torch.Tensor):
+        """The same layer over prompts laid out back to back: ``hidden`` ``[tokens, H]``, no padded rows.
+
+        Differentiable through the kernels.  Queries and keys are turned in FP32 and rounded once
+        (``forward`` multiplies by tables of the activations' type)."""
+        to_q, to_k, to_v, to_out, norm_q, norm_k = self.self_attn.parts()
+        heads, kv_heads, dim = self.num_attention_heads, self.num_key_value_heads, self.head_dim
+        normalized = self.input_layernorm(hidden)
+        joint = ops.joint_linear(normalized, (to_q, to_k, to_v))
+        query, key, value = (to_q(normalized), to_k(normalized), to_v(normalized)) if joint is None else \
+            joint.split((heads * dim, kv_heads * dim, kv_heads * dim), dim=-1)
+        query = norm_q(query.unflatten(-1, (heads, dim)))
+        key = norm_k(key.unflatten(-1, (kv_heads, dim)))
+        value = value.unflatten(-1, (kv_heads, dim))
+        query, key = ops.rotary_embed(query, key, positions, frequencies)
+        output = ops.packed_attention(query, key, value, offsets)
+        residual = hidden + to_out(output.flatten(-2))
+        return residual + self.mlp(self.post_attention_layernorm(residual)), key, value
+
+
 class Cosmos3GenLayer(nn.Module):
     """Generation-tower layer over a list of token chunks and one attention policy."""
 

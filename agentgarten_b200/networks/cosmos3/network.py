@@ -38,6 +38,7 @@ import torch
 from einops import rearrange
 from torch import nn
 
+from agentgarten_b200 import ops
 from agentgarten_b200.parallel.network import ParallelNetwork
 from agentgarten_b200.protocols import HistoryWindow
 
@@ -120,6 +121,42 @@ class Cosmos3TextEncoder(ParallelNetwork):
         for layer in self.layers:
             hidden, key, value = layer(hidden, rope)
             per_layer.append((key, value))
+        return TextContext(keys=tuple(k for k, _ in per_layer), values=tuple(v for _, v in per_layer),
+                           valid_lengths=torch.tensor(lengths, device=device), lengths=lengths)
+
+
+    def encode_packed(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, *,
+                      scaling: str | None = None, factor: float = 1.0,
+                      trained_positions: int | None = None) -> TextContext:
+        """``forward`` without its padded rows: the prompts run back to back through the layers.
+
+        The keys and values behind a prompt's end are zeros (``forward`` leaves those of its padding
+        there; nothing reads either).  ``scaling`` stretches the rotary positions for prompts beyond
+        the trained lengths (:func:`agentgarten_b200.ops.rotary_frequencies`).  Differentiable, for a
+        text tower that is trained.
+        """
+        config, device = self.config, self.embed_tokens.weight.device
+        prompts = [prompt.to(device) for prompt in pack_text_rows(input_ids, attention_mask, config.special_tokens)]
+        lengths = tuple(int(prompt.numel()) for prompt in prompts)
+        width = max(max(lengths), int(config.text_bucket_tokens or 0))
+        sizes = torch.tensor(lengths)
+        starts = torch.cat((sizes.new_zeros(1), sizes.cumsum(0)))
+        index = torch.arange(int(starts[-1]))
+        positions = (index - starts[:-1].repeat_interleave(sizes)).to(device)
+        slots = (torch.arange(len(lengths)) * width).repeat_interleave(sizes).to(device) + positions  # in the context
+        frequencies = ops.rotary_frequencies(config.head_dim, config.rope_theta, scaling=scaling, factor=factor,
+                                             trained_positions=trained_positions, device=device)
+        offsets = starts.to(device=device, dtype=torch.int32)
+        hidden = self.embed_tokens(torch.cat(prompts))
+
+        def placed(rows: torch.Tensor) -> torch.Tensor:
+            table = rows.new_zeros(len(lengths) * width, *rows.shape[1:]).index_copy(0, slots, rows)
+            return table.unflatten(0, (len(lengths), width))
+
+        per_layer = []
+        for layer in self.layers:
+            hidden, key, value = layer.forward_packed(hidden, positions, frequencies, offsets)
+            per_layer.append((placed(key), placed(value)))
         return TextContext(keys=tuple(k for k, _ in per_layer), values=tuple(v for _, v in per_layer),
                            valid_lengths=torch.tensor(lengths, device=device), lengths=lengths)
 

@@ -410,3 +410,201 @@ def test_gradients_of_gradients_are_refused():
         (grad,) = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiable once"):
             grad.sum().backward()
+
+
+# ------------------------------------------------------------------------------ as they are used
+@pytest.mark.parametrize("interleaved,turned,scaling", [(False, 128, None), (True, 64, "yarn")])
+def test_prompt_then_tokens_against_a_cache(interleaved, turned, scaling):
+    """Prompts turned and attended in one packed batch, then single tokens that are turned, written
+    into a cache with room behind every prompt and attended against it: every row is the row of the
+    whole sequence."""
+    lengths, extra, room, heads, kv_heads, dim = [130, 5, 700], 3, 720, 8, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(12)
+    whole = [n + extra for n in lengths]
+    q, k, v = (torch.randn(sum(whole), h, dim, device=DEV, generator=g).bfloat16() for h in (heads, kv_heads, kv_heads))
+    f = ops.rotary_frequencies(turned, 5e6, scaling=scaling, factor=4.0, trained_positions=512, device=DEV)
+    starts = _offsets(whole).tolist()
+    positions = torch.cat([torch.arange(n, device=DEV) for n in whole])
+    qr, kr = ops.rotary_embed(q, k, positions, f, interleaved=interleaved)
+    spans = [(a, n, a, n) for a, n in zip(starts, whole)]
+    value, bound = oracle.attention(qr, kr, v, spans, dim ** -0.5)["out"]
+
+    prompt = torch.cat([torch.arange(a, a + n, device=DEV) for a, n in zip(starts, lengths)])
+    pq, pk = ops.rotary_embed(q[prompt], k[prompt], positions[prompt], f, interleaved=interleaved)
+    assert torch.equal(pq, qr[prompt]) and torch.equal(pk, kr[prompt])
+    out = ops.packed_attention(pq, pk, v[prompt], _offsets(lengths))
+    oracle.assert_close(out, value[prompt], bound[prompt])
+
+    cache = [torch.full((room * 3, kv_heads, dim), float("nan"), device=DEV, dtype=BF16) for _ in range(2)]
+    rows = torch.cat([torch.arange(s * room, s * room + n, device=DEV) for s, n in enumerate(lengths)])
+    cache[0][rows], cache[1][rows] = pk, v[prompt]
+    at = torch.arange(0, 3 * room + 1, room, dtype=torch.int32, device=DEV)
+    filled = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    one = _offsets([1, 1, 1])
+    for step in range(extra):
+        new = torch.tensor([a + n + step for a, n in zip(starts, lengths)], device=DEV)
+        tq, tk = ops.rotary_embed(q[new], k[new], positions[new], f, interleaved=interleaved)
+        slot = (at[:-1] + filled).long()
+        cache[0][slot], cache[1][slot] = tk, v[new]
+        filled += 1
+        out = ops.packed_attention(tq, *cache, one, at, k_lengths=filled)
+        oracle.assert_close(out, value[new], bound[new])
+    assert _status() == 0
+
+
+def _tower(dtype):
+    from helpers import tiny_conditioner, tiny_config
+
+    config = tiny_config(hidden_size=512, num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+                         mrope_section=(24, 20, 20), text_bucket_tokens=64)
+    return tiny_conditioner(config, dtype=dtype).text_encoder
+
+
+def test_text_tower_on_packed_prompts():
+    """bf16 on the kernels against the same weights in 64 bits: no further off than the padded tower,
+    whose roundings are the same or more, up to what a different draw of roundings gives."""
+    encoder = _tower(BF16)
+    ids = torch.randint(3, 128, (5, 50))
+    valid = torch.arange(50)[None] < torch.tensor([50, 1, 33, 17, 49])[:, None]
+    want = _tower(BF16).double().encode_packed(ids, valid)
+    encoder.to(DEV)
+    before = native.launches()
+    packed = encoder.encode_packed(ids.to(DEV), valid.to(DEV))
+    assert native.launches() > before
+    padded = encoder(ids.to(DEV), valid.to(DEV))
+    for mine, theirs, exact in zip((*packed.keys, *packed.values), (*padded.keys, *padded.values),
+                                   (*want.keys, *want.values)):
+        off = [0.0, 0.0]
+        for row, n in enumerate(packed.lengths):
+            for i, t in enumerate((mine, theirs)):
+                off[i] += float((t[row, :n].double().cpu() - exact[row, :n]).square().sum())
+            assert not mine[row, n:].any()
+        assert off[0] ** 0.5 <= 1.5 * off[1] ** 0.5
+    assert _status() == 0
+
+
+def test_text_tower_trains_on_packed_prompts():
+    """Gradients of all layers in bf16 on the kernels against 64 bits on the CPU."""
+    ids = torch.randint(3, 128, (3, 40))
+    valid = torch.arange(40)[None] < torch.tensor([40, 9, 26])[:, None]
+    grads, yard = [], None
+    for encoder, device in ((_tower(BF16).double(), "cpu"), (_tower(BF16).to(DEV), DEV)):
+        encoder.requires_grad_(True)
+        context = encoder.encode_packed(ids.to(device), valid.to(device))
+        weights = [layer.self_attn.to_k.weight for layer in encoder.layers] + [encoder.embed_tokens.weight]
+        loss = sum(t.double().square().sum() for t in (*context.keys, *context.values))
+        grads.append([g.double().cpu() for g in torch.autograd.grad(loss, weights, retain_graph=True)])
+        if yard is None:
+            # The keys are normalised, so the sum of their squares is constant and its exact gradient next
+            # to nothing: a rounding's size goes by the terms that cancel.  A rounding is a change of
+            # 2^-8 of them in a direction of its own; what the sizes |2 t| of the loss's gradient come to
+            # in random directions is the gradient of sum s |2 t| t with t of the factor held.
+            g = torch.Generator().manual_seed(9)
+            other = sum((t * (2 * t.detach().abs() * torch.randn(t.shape, generator=g, dtype=t.dtype).sign())).sum()
+                        for t in (*context.keys, *context.values))
+            yard = [x.norm() for x in torch.autograd.grad(other, weights)]
+    # about 20 roundings of 2^-8 on the way through two layers and back, adding up as a random walk,
+    # and bf16 weight gradients
+    for a, b, size in zip(*grads, yard):
+        assert (a - b).norm() <= 20 ** 0.5 * 2.0 ** -8 * 2 * max(size, a.norm())
+
+
+# -------------------------------------------------------------------------------- graphs, streams
+def test_calls_replay_in_graphs_with_other_lengths():
+    """Captured calls read their lengths at replay: the same graph serves other lengths, also two graphs
+    side by side on two streams."""
+    def state(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        q = torch.randn(400, 8, 128, device=DEV, generator=g).bfloat16()
+        k, v = (torch.randn(4000, 2, 128, device=DEV, generator=g).bfloat16() for _ in range(2))
+        return q, k, v
+
+    def spans(qo, ko, kl):
+        qo, ko, kl = qo.tolist(), ko.tolist(), kl.tolist()
+        return [(a, b - a, c, n) for a, b, c, n in zip(qo, qo[1:], ko, kl)]
+
+    graphs = []
+    for seed, lengths in ((1, [100, 300]), (2, [1] * 400)):
+        q, k, v = state(seed)
+        n = len(lengths)
+        room = 4000 // n
+        qo, ko = _offsets(lengths), _offsets([room] * n)
+        kl = torch.full((n,), room, dtype=torch.int32, device=DEV)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.packed_attention(q, k, v, qo, ko, k_lengths=kl)
+        graphs.append((graph, q, k, v, qo, ko, kl, out))
+    for shrink in (0, 7):
+        for _, _, _, _, _, _, kl, _ in graphs:
+            kl -= shrink
+        torch.cuda.synchronize()
+        for _ in range(3):
+            streams = [torch.cuda.Stream() for _ in graphs]
+            for stream, entry in zip(streams, graphs):
+                with torch.cuda.stream(stream):
+                    entry[0].replay()
+            torch.cuda.synchronize()
+        for _, q, k, v, qo, ko, kl, out in graphs:
+            oracle.assert_close(out, *oracle.attention(q, k, v, spans(qo, ko, kl), 128 ** -0.5)["out"])
+    assert _status() == 0
+
+
+def test_training_step_replays_in_a_graph():
+    q, k, v, qo, ko, kl, spans = _case([130, 70], [130, 70], 4, 2, 64, BF16, seed=6)
+    f = ops.rotary_frequencies(64, 1e4, device=DEV)
+    positions = torch.cat([torch.arange(n, device=DEV) for n in (130, 70)])
+    grad = torch.randn_like(q)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        a, b = ops.rotary_embed(q, k, positions, f)
+        out = ops.packed_attention(a, b, v, qo)
+        return out.detach(), *torch.autograd.grad(out, leaves, grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    with torch.no_grad():
+        q.copy_(q.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in captured]
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+    assert _status() == 0
+
+
+def test_calls_on_another_stream_and_their_gradients():
+    q, k, v, qo, ko, kl, spans = _case([300], [300], 4, 2, 128, BF16, seed=7)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    grad = torch.randn_like(q)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        out = ops.packed_attention(q, k, v, qo)
+        grads = torch.autograd.grad(out, leaves, grad)
+    stream.synchronize()
+    want = oracle.attention(q.detach(), k.detach(), v.detach(), spans, 128 ** -0.5, grad)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        oracle.assert_close(got, *want[name], name)
+
+
+def test_many_sequences():
+    """More sequences than are ranked by length, and more than a step of the searches."""
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 40, (1500,), generator=g).tolist()
+    _check_forward(lengths, lengths, 4, 2, 64, BF16, behind=9)
+    _check_gradients(lengths[:300], lengths[:300], 4, 2, 64, BF16, behind=9)
+    _check_forward([1] * 1500, [n + 1 for n in lengths], 8, 2, 64, FP16, room=2, behind=1)
+    rows = torch.randint(0, 3, (1500,), generator=g).tolist()
+    _check_forward(rows, [n + 2 for n in lengths], 8, 2, 64, FP16, room=2, behind=1)

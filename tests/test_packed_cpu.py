@@ -152,3 +152,74 @@ def test_attention_refusals():
             call(q_offsets=torch.tensor(bad, dtype=torch.int32))
     with pytest.raises(ValueError, match="offsets"):
         call(k_lengths=torch.tensor([4, 4], dtype=torch.int32))
+
+
+# ------------------------------------------------------------------------------- the text tower
+def _prompts():
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(3, 128, (3, 12), generator=g)
+    valid = torch.arange(12)[None] < torch.tensor([12, 3, 7])[:, None]
+    return ids, valid
+
+
+def test_packed_prompts_give_the_text_towers_context():
+    from helpers import tiny_conditioner
+
+    encoder = tiny_conditioner().text_encoder.double()
+    ids, valid = _prompts()
+    padded, packed = encoder(ids, valid), encoder.encode_packed(ids, valid)
+    assert packed.lengths == padded.lengths and torch.equal(packed.valid_lengths, padded.valid_lengths)
+    for mine, theirs in zip((*packed.keys, *packed.values), (*padded.keys, *padded.values)):
+        assert mine.shape == theirs.shape
+        for row, (a, b) in enumerate(zip(mine, theirs)):
+            n = packed.lengths[row]
+            # the padded tower's angles are FP32: off by 14 * 2^-24 at the last position, in values of
+            # order 1 and through two layers
+            torch.testing.assert_close(a[:n], b[:n], rtol=0, atol=14 * 2.0 ** -24 * 16)
+            assert not a[n:].any()
+
+
+def test_packed_prompts_train_the_text_tower():
+    from helpers import tiny_conditioner
+
+    encoder = tiny_conditioner().text_encoder.double()
+    encoder.requires_grad_(True)
+    ids, valid = _prompts()
+    weights = [layer.self_attn.to_k.weight for layer in encoder.layers] + [encoder.embed_tokens.weight]
+
+    def value():
+        context = encoder.encode_packed(ids, valid, scaling="yarn", factor=2.0, trained_positions=64)
+        return sum((t * t.detach().sign()).sum() for t in (*context.keys, *context.values))
+
+    grads = torch.autograd.grad(value(), weights)
+    g = torch.Generator().manual_seed(5)
+    with torch.no_grad():
+        steps = [torch.randn(w.shape, generator=g, dtype=w.dtype) for w in weights]
+        slope = sum((a * b).sum() for a, b in zip(grads, steps))
+        h = 1e-7
+        ends = []
+        for sign in (1, -2):
+            for w, s in zip(weights, steps):
+                w += sign * h * s
+            ends.append(value())
+    # differences of a smooth function: h^2 terms and 2^-53 of its size over h
+    assert abs((ends[0] - ends[1]) / (2 * h) - slope) < 1e-4 * abs(slope) + 1e-9 / h * 2.0 ** -20 * abs(ends[0])
+
+
+def test_conditioner_packs_prompts_when_asked():
+    from helpers import synthetic_batch, tiny_conditioner
+
+    conditioner = tiny_conditioner()
+    batch = conditioner.encode(synthetic_batch(batch=2), training=False)
+    plain = conditioner.condition(batch).text
+    conditioner.pack_prompts = True
+    packed = conditioner.condition(batch).text
+    assert packed.lengths == plain.lengths
+    for a, b in zip(packed.keys, plain.keys):
+        n = packed.lengths[0]
+        torch.testing.assert_close(a[:, :n], b[:, :n], rtol=0, atol=1e-4)
+    conditioner.cache_text_contexts = True
+    again = conditioner.condition(batch).text
+    assert conditioner.condition(batch).text is again
+    conditioner.pack_prompts = False
+    assert conditioner.condition(batch).text is not again
