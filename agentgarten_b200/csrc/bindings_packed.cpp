@@ -249,13 +249,14 @@ int rows_chunk(const agb::PackedArgs& a, int sms) {
 // tile's work (about 0.9 us): the longest CTA, twice the mean's, or all of the work over the SMs;
 // then the join, about 4 us and the partial results' way to memory and back.
 int tile_splits(const agb::PackedArgs& a, int sms) {
-  const bool paired = (a.hq / a.hkv) % 2 == 0;
-  const double step = paired ? 128 : 256;
+  int fold = 1;
+  while (fold < 16 && (a.hq / a.hkv) % (2 * fold) == 0) fold *= 2;
+  const double step = 256 / fold;
   const double rows = double(a.total_q) / a.sequences, keys = double(a.total_k) / a.sequences;
   const double pieces = std::ceil(rows / step);
   const double seen = std::max(keys - rows / 2, rows / 2);  // of a row, on average
   const double tiles = std::ceil(seen / 128);
-  const double all = a.sequences * pieces * (paired ? a.hq / 2 : a.hq) * tiles / sms;
+  const double all = a.sequences * pieces * (a.hq / fold) * tiles / sms;
   const double partial = double(a.total_q) * a.hq * a.dim * 8 / 6.5e6 / 0.9;
   int best = 1;
   double best_cost = std::max(2 * tiles, all);
@@ -381,7 +382,7 @@ c10::optional<Tensor> packed_attention(const Tensor& query, const Tensor& key, c
   if (std::max(query.size(0), key.size(0)) >= (int64_t(1) << 31) - 256) refuse_value(op, "rows are counted in 32 bits");
   const double scale = scale_given.has_value() ? *scale_given : 1.0 / std::sqrt(double(dim));
   if (!(scale > 0) || std::isinf(scale)) refuse_value(op, "scale is positive");
-  if ((type != torch::kBFloat16 && type != torch::kHalf) || dim % 8 || dim > 128 || has_tangent(query) ||
+  if ((type != torch::kBFloat16 && type != torch::kHalf) || dim % 8 || dim > 128 || heads * dim >= (1 << 24) || has_tangent(query) ||
       has_tangent(key) || has_tangent(value))
     return c10::nullopt;
   if (at::GradMode::is_enabled() && (wants_grad(query) || wants_grad(key) || wants_grad(value)))

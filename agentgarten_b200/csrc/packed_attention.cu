@@ -4,9 +4,9 @@
 //
 // A CTA works through items (piece of a sequence's queries, two score tiles, key range), which come in the
 // order of falling length: it is launched for one and takes over further ones that have not started yet
-// (one CTA fits an SM).  The two tiles of 128 rows
-// are two query heads that share a key head, or, when a key head has an odd number of query heads,
-// two neighbouring tiles of one head; both read the same K and V tiles.
+// (one CTA fits an SM).  The rows of a tile are (query row, head) pairs of up to 16 heads that share a
+// key head; the two tiles of an item are neighbours and read the same K and V tiles.  (With a tile of
+// 128 rows of one head, sixteen prompts of 14 to 514 rows had a third more tiles.)
 //   warps 0-3  softmax of tile 0: one query row per thread; then its output
 //   warps 4-7  softmax of tile 1
 //   warp 8     TMA producer (K and V through rings of two stages, which run on from item to item)
@@ -64,19 +64,19 @@ struct FwdParams {
   float* lse;
   float* part_out; float* part_lse;
   int hq, dim, group, splits;
-  int head_units;   // items side by side for one piece: hq / 2 (pairs of heads) or hq
-  int paired;       // 1: the tiles are two heads, 0: two neighbouring row tiles
+  int shift;        // heads folded into a tile's rows: 1 << shift
+  int head_units;   // items side by side for one piece: hq >> shift
   float scale_log2;
   int* status;
 };
 
-// What the roles need of an item.  Per tile: head, first row within the sequence, rows, key tiles (from
-// the range's first on).
+// What the roles need of an item.  Per tile: first query row within the sequence, query rows, key tiles
+// (from the range's first on).
 enum : int { ITEM_END = 0, ITEM_TILES = 1, ITEM_UNCOVERED = 2 };
 struct Item {
   int kind, split;
-  int head[2], first[2], rows[2], tiles[2];
-  int kv_head, q0, k0, query_rows, keys;
+  int first[2], rows[2], tiles[2];
+  int head0, kv_head, q0, k0, query_rows, keys;
   int lo, n;        // range of key tiles
   int last_valid;   // keys that exist in the range's last tile (128 or more: all)
 };
@@ -84,22 +84,22 @@ constexpr int ITEM_READERS = 11;  // eight softmax warps, producer, issuer, clea
 
 __device__ inline Item make_item(const PackedSpan& span, const FwdParams& p, int head_unit, int split) {
   Item item{};
-  const int step = p.paired ? ROWS : 2 * ROWS;
+  const int step = ROWS >> p.shift;  // query rows of a tile
   item.kind = span.unit_in_sequence == -2 ? ITEM_UNCOVERED : ITEM_TILES;
   item.split = split;
   item.q0 = span.q0;
   item.k0 = span.k0;
   item.query_rows = span.rows;
   item.keys = span.keys;
+  item.head0 = head_unit << p.shift;
+  item.kv_head = item.head0 / p.group;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    item.head[t] = p.paired ? 2 * head_unit + t : head_unit;
-    item.first[t] = span.unit_in_sequence * step + (p.paired ? 0 : t * ROWS);
-    item.rows[t] = item.kind == ITEM_TILES ? max(0, min(ROWS, span.rows - item.first[t])) : 0;
+    item.first[t] = (2 * span.unit_in_sequence + t) * step;
+    item.rows[t] = item.kind == ITEM_TILES ? max(0, min(step, span.rows - item.first[t])) : 0;
     const int seen = min(span.keys, span.keys - span.rows + item.first[t] + item.rows[t]);  // keys of the last row
     item.tiles[t] = item.rows[t] == 0 || seen <= 0 ? 0 : (seen + ROWS - 1) / ROWS;
   }
-  item.kv_head = item.head[0] / p.group;
   const int most = max(item.tiles[0], item.tiles[1]);
   const int per = (most + p.splits - 1) / p.splits;
   item.lo = min(most, split * per);
@@ -199,7 +199,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           if (!item_wait(i, kTimeoutProducer)) { ok = false; break; }
           const Item& it = items[i & 1];
           const int kind = it.kind, n = it.n, kv_head = it.kv_head, q0 = it.q0, row0 = it.k0 + it.lo * ROWS;
-          const int head[2] = {it.head[0], it.head[1]}, first[2] = {it.first[0], it.first[1]};
+          const int head0 = it.head0, first[2] = {it.first[0], it.first[1]};
           const bool there[2] = {it.tiles[0] > 0, it.tiles[1] > 0}, ragged = it.last_valid < ROWS;
           item_free(i);
           if (kind == ITEM_END) break;
@@ -214,7 +214,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           for (int t = 0; t < 2; ++t)
             if (there[t])
               for (int a = 0; a < ATOMS; ++a)
-                tma_load_3d(sQ + t * TILE_BYTES + a * HALF_BYTES, &tm_q, q_full, a * 64, head[t], q0 + first[t]);
+                tma_load_3d(sQ + t * TILE_BYTES + a * HALF_BYTES, &tm_q, q_full, a * 64, head0, q0 + first[t]);
           for (int j = 0; j < n && ok; ++j, ++loads) {
             const int st = loads % KV_STAGES;
             const uint32_t ph = ((loads / KV_STAGES) & 1) ^ 1;
@@ -326,7 +326,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const int side = p.head_units * p.splits;  // blocks of one piece, splits fastest
           const int piece = divide(int(unit), side), rest = int(unit) - piece * side;
           const int head_unit = divide(rest, p.splits), split = rest - head_unit * p.splits;
-          const PackedSpan span = find_piece(piece, p.paired ? ROWS : 2 * ROWS, false, p.q_offsets, p.k_offsets,
+          const PackedSpan span = find_piece(piece, 2 * ROWS >> p.shift, false, p.q_offsets, p.k_offsets,
                                              p.k_lengths, p.sequences, p.total_q, p.total_k,
                                              head_unit == 0 && split == 0 ? p.status : nullptr);
           work = !(span.unit_in_sequence == -1 || (span.unit_in_sequence == -2 && span.rows == 0));
@@ -386,25 +386,25 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     for (int i = 0; ok; ++i) {
       if (!item_wait(i, kTimeoutSoftmax)) break;
       const Item& it = items[i & 1];
-      const int kind = it.kind, my_tiles = it.tiles[t], my_rows = it.rows[t], my_head = it.head[t], split = it.split;
-      const int q_row = it.q0 + it.first[t];     // first row of the tile
-      // keys that this row, and the warp's first row, see, from the first key of the range on
+      const int kind = it.kind, my_tiles = it.tiles[t], my_rows = it.rows[t], head0 = it.head0, split = it.split;
+      const int q_row = it.q0 + it.first[t];     // first query row of the tile
+      // keys that this row, and the warp's first and last row, see, from the first key of the range on
       const int it_keys = it.keys - it.lo * ROWS;
       const int before = it_keys - it.query_rows + it.first[t] + 1;
-      const int seen = min(it_keys, before + my_row);
-      const int seen_warp = min(it_keys, before + quarter * 32);
+      const int seen = min(it_keys, before + (my_row >> p.shift));
+      const int seen_warp = min(it_keys, before + (quarter * 32 >> p.shift));
+      const int seen_most = min(it_keys, before + (quarter * 32 + 31 >> p.shift));
       const int uncovered0 = it.q0, uncovered = it.query_rows;
       __syncwarp();
       if (lane == 0) item_free(i);
       if (kind == ITEM_END) break;
       if (kind == ITEM_UNCOVERED) {  // zeros (the join writes them for split launches)
-        const int words = p.dim / 8;
-        if (p.splits == 1 && (p.paired || t == 0))
-          for (int w = my_row; w < uncovered * words; w += ROWS) {
-            uint16_t* dst = static_cast<uint16_t*>(p.out) +
-                            ((int64_t(uncovered0) + w / words) * p.hq + my_head) * p.dim + (w % words) * 8;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-          }
+        const int words = (p.dim << p.shift) / 8;  // of the item's heads in a row
+        if (p.splits == 1)
+          for (int w = t * ROWS + my_row; w < uncovered * words; w += 2 * ROWS)
+            store16(static_cast<uint16_t*>(p.out) + ((int64_t(uncovered0) + w / words) * p.hq + head0) * p.dim +
+                        (w % words) * 8,
+                    make_uint4(0, 0, 0, 0));
         continue;
       }
       float m_ref = -INFINITY;                   // reference maximum (log2 domain)
@@ -494,7 +494,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             hand_over(packed, c);
           }
         } else {
-          const int most = min(it_keys - j * ROWS, sure + 31);
+          const int most = seen_most - j * ROWS;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t packed[32];
@@ -519,9 +519,10 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       tc_fence_after_sync();
       const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
       const bool partial = p.splits > 1;
-      const int live = min(32, my_rows - quarter * 32);   // rows of this warp
-      const int64_t row = int64_t(q_row) + quarter * 32;  // its first
-      const int64_t at = (partial ? int64_t(split) * p.total_q : 0) * p.hq + row * p.hq + my_head;
+      const int live = min(32, (my_rows << p.shift) - quarter * 32);    // rows of this warp
+      const int64_t row = int64_t(q_row) + (quarter * 32 >> p.shift);   // the query row of its first
+      const int head = head0 + (quarter * 32 & ((1 << p.shift) - 1));   // and the head (folds are at most 32)
+      const int64_t at = ((partial ? int64_t(split) * p.total_q : 0) + row) * p.hq + head;
       if (live > 0 && !(partial && my_tiles == 0)) {
         // 128 bytes of every row at a time: 64 elements, or 32 of a partial result
 #pragma unroll 1
@@ -546,7 +547,7 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                                  __float_as_uint(__uint_as_float(o[h][g * 4 + 2]) * inv),
                                  __float_as_uint(__uint_as_float(o[h][g * 4 + 3]) * inv)));
               flush_rows(stage, reinterpret_cast<uint8_t*>(p.part_out + at * p.dim + c * 64 + h * 32),
-                         int64_t(p.hq) * p.dim * 4, (p.dim - c * 64 - h * 32) * 4, live, lane);
+                         p.hq * p.dim * 4, p.dim * 4, p.shift, (p.dim - c * 64 - h * 32) * 4, live, lane);
             }
           } else {
 #pragma unroll
@@ -560,14 +561,15 @@ packed_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               put16(stage_word(stage, lane, g), v);
             }
             flush_rows(stage, reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p.out) + at * p.dim + c * 64),
-                       int64_t(p.hq) * p.dim * 2, (p.dim - c * 64) * 2, live, lane);
+                       p.hq * p.dim * 2, p.dim * 2, p.shift, (p.dim - c * 64) * 2, live, lane);
           }
         }
       }
       if (lane < live) {
         const float log_sum = l_sum == 0.f ? -INFINITY : m_ref + log2f(l_sum);
-        if (partial) p.part_lse[at + int64_t(lane) * p.hq] = log_sum;
-        else if (p.lse) p.lse[int64_t(my_head) * p.total_q + row + lane] = log_sum * 0.6931471805599453f;
+        const int down = lane >> p.shift, across = lane & ((1 << p.shift) - 1);
+        if (partial) p.part_lse[at + int64_t(down) * p.hq + across] = log_sum;
+        else if (p.lse) p.lse[int64_t(head + across) * p.total_q + row + down] = log_sum * 0.6931471805599453f;
       }
     }
   }
@@ -634,11 +636,11 @@ cudaError_t launch_tiles(const PackedArgs& a, const CUtensorMap& tq, const CUten
   p.total_q = a.total_q; p.total_k = a.total_k;
   p.out = a.out; p.lse = a.lse; p.part_out = a.part_out; p.part_lse = a.part_lse;
   p.hq = a.hq; p.dim = a.dim; p.group = a.hq / a.hkv; p.splits = a.splits;
-  p.paired = p.group % 2 == 0;
-  p.head_units = p.paired ? a.hq / 2 : a.hq;
+  p.shift = fold_shift(p.group);
+  p.head_units = a.hq >> p.shift;
   p.scale_log2 = a.scale * LOG2E;
   p.status = a.status;
-  const int step = p.paired ? ROWS : 2 * ROWS;
+  const int step = 2 * ROWS >> p.shift;
   const int64_t units = (a.total_q / step + a.sequences + 1) * p.head_units * p.splits;
   const int64_t blocks = (a.total_q * a.hq + 7) / 8;
   if (units > 2147483647ll || blocks > 2147483647ll) {
@@ -654,20 +656,21 @@ cudaError_t launch_tiles(const PackedArgs& a, const CUtensorMap& tq, const CUten
 
 }  // namespace
 
-// A [rows, heads, dim] tensor in boxes of 64 elements x 1 head x 128 rows; elements behind dim read as zero.
+// A [rows, heads, dim] tensor in boxes of 64 elements x `fold` heads x 128 / fold rows; elements behind dim read
+// as zero.
 bool make_packed_map(CUtensorMap* map, const void* base, int dim, int heads, int64_t rows, int64_t head_stride,
-                     int64_t row_stride) {
+                     int64_t row_stride, int fold) {
   const uint64_t dims[3] = {uint64_t(dim), uint64_t(heads), uint64_t(rows)};
   const uint64_t strides[2] = {uint64_t(head_stride) * 2, uint64_t(row_stride) * 2};
-  const uint32_t box[3] = {64, 1, 128};
+  const uint32_t box[3] = {64, uint32_t(fold), uint32_t(128 / fold)};
   return encode_tensor_map_16bit(map, base, 3, dims, strides, box);
 }
 
 cudaError_t packed_attention_tiles(const PackedArgs& a, cudaStream_t stream) {
   CUtensorMap tq, tk, tv;
-  if (!make_packed_map(&tq, a.q, a.dim, a.hq, a.total_q, a.q_head, a.q_row) ||
-      !make_packed_map(&tk, a.k, a.dim, a.hkv, a.total_k, a.k_head, a.k_row) ||
-      !make_packed_map(&tv, a.v, a.dim, a.hkv, a.total_k, a.v_head, a.v_row))
+  if (!make_packed_map(&tq, a.q, a.dim, a.hq, a.total_q, a.q_head, a.q_row, 1 << fold_shift(a.hq / a.hkv)) ||
+      !make_packed_map(&tk, a.k, a.dim, a.hkv, a.total_k, a.k_head, a.k_row, 1) ||
+      !make_packed_map(&tv, a.v, a.dim, a.hkv, a.total_k, a.v_head, a.v_row, 1))
     return cudaErrorInvalidValue;
   if (a.dim <= 64)
     return a.fp16 ? launch_tiles<64, true>(a, tq, tk, tv, stream) : launch_tiles<64, false>(a, tq, tk, tv, stream);

@@ -4,10 +4,10 @@
 //   dq = scale ds k,  dk = scale ds^T q,  dv = p^T dO
 //
 // Two kernels, both without atomics, so a gradient is the same on every run:
-//   packed_dq    one CTA per (128 query rows of a sequence, query head) walks the key tiles up to its
-//                diagonal: S = Q K^T, dP = dO V^T, dQ += dS K.  It also writes delta for
+//   packed_dq    one CTA per 128 (query row, head) pairs of up to 16 heads that share a key head walks the
+//                key tiles up to its diagonal: S = Q K^T, dP = dO V^T, dQ += dS K.  It also writes delta for
 //   packed_dkdv  one CTA per (128 key rows of a sequence, key head) walks the query tiles that see
-//                them, for the query heads of its group in turn:
+//                them, 128 (query row, head) pairs at a time:
 //                S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
 // Shared heads are summed in the accumulators, in FP32.  P and dS are rounded to the tensors' type
 // on their way into the tensor core (scale stays out of dS and is applied to the sums, which keeps
@@ -25,7 +25,7 @@
 namespace agb {
 
 bool make_packed_map(CUtensorMap* map, const void* base, int dim, int heads, int64_t rows, int64_t head_stride,
-                     int64_t row_stride);
+                     int64_t row_stride, int fold);
 
 namespace {
 
@@ -46,7 +46,8 @@ struct BwdParams {
   float* delta;         // [hq, total_q]
   void* dq; void* dk; void* dv;  // dense
   int hq, hkv, group, dim;
-  int share;            // CTAs (a cluster) that share the query heads of a key tile
+  int shift;            // heads folded into a query tile's rows: 1 << shift
+  int share;            // CTAs (a cluster) that share the query tiles of a key tile
   float scale, scale_log2;
   int* status;
 };
@@ -60,8 +61,8 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
 // stage.  Without `filled` (uniform over the warp) the accumulator holds nothing and zeros are
 // written; so are the rows that are not `live`.
 template <bool FP16>
-__device__ __forceinline__ void store_columns(uint16_t* dst, int64_t pitch, uint32_t taddr, int left, float scale, int rows,
-                                              bool filled, bool live, uint32_t stage, int lane) {
+__device__ __forceinline__ void store_columns(uint16_t* dst, int pitch, int head_pitch, int shift, uint32_t taddr, int left,
+                                              float scale, int rows, bool filled, bool live, uint32_t stage, int lane) {
   uint32_t o[2][32];
   if (filled) {
     tmem_ld_32x32(taddr, o[0]);
@@ -84,7 +85,7 @@ __device__ __forceinline__ void store_columns(uint16_t* dst, int64_t pitch, uint
     v.w = pack16<FP16>(__uint_as_float(x[6]) * scale, __uint_as_float(x[7]) * scale);
     put16(stage_word(stage, lane, g), v);
   }
-  flush_rows(stage, reinterpret_cast<uint8_t*>(dst), pitch * 2, left * 2, rows, lane);
+  flush_rows(stage, reinterpret_cast<uint8_t*>(dst), pitch * 2, head_pitch * 2, shift, left * 2, rows, lane);
 }
 
 // Probabilities of a pair of scores, one pair in four on the FMA pipe (see exp2_fma).
@@ -138,14 +139,15 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   int* span_smem = reinterpret_cast<int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = int(blockIdx.x % unsigned(p.hq));
-  const int unit = int(blockIdx.x / unsigned(p.hq));
-  const int kv_head = head / p.group;
+  const int head_units = p.hq >> p.shift, unit = divide(int(blockIdx.x), head_units);
+  const int head0 = (int(blockIdx.x) - unit * head_units) << p.shift;
+  const int kv_head = head0 / p.group;
+  const int step = ROWS >> p.shift;  // query rows of the tile
   const WaitGuard guard{abort_flag, p.status};
 
   if (warp == 0) {
-    const PackedSpan span = find_piece(unit, ROWS, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
-                                       p.total_q, p.total_k, head == 0 ? p.status : nullptr);
+    const PackedSpan span = find_piece(unit, step, false, p.q_offsets, p.k_offsets, p.k_lengths, p.sequences,
+                                       p.total_q, p.total_k, head0 == 0 ? p.status : nullptr);
     if (lane == 0) *reinterpret_cast<PackedSpan*>(span_smem) = span;
   }
   if (warp == 1 && lane == 0) {
@@ -179,8 +181,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   constexpr uint32_t C_S = 0, C_DP = 256, C_DQ = 384;
 
   const bool covered = span.unit_in_sequence >= 0;
-  const int first = covered ? span.unit_in_sequence * ROWS : 0;
-  const int rows = covered ? min(ROWS, span.rows - first) : 0;
+  const int first = covered ? span.unit_in_sequence * step : 0;
+  const int rows = covered ? min(step, span.rows - first) : 0;
   const int q_row = span.q0 + first;
   const int reach = span.keys - span.rows + first;  // row i of the tile sees the keys up to reach + i
   const int seen_last = covered ? min(span.keys, reach + rows) : 0;
@@ -193,8 +195,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       bool ok = true;
       if (lane == 0) {
         mbar_expect_tx(q_full, 2 * TILE_BYTES);
-        load_tile<ATOMS>(sQ, &tm_q, q_full, head, q_row);
-        load_tile<ATOMS>(sdO, &tm_do, q_full, head, q_row);
+        load_tile<ATOMS>(sQ, &tm_q, q_full, head0, q_row);
+        load_tile<ATOMS>(sdO, &tm_do, q_full, head0, q_row);
         for (int j = 0; j < n_tiles && ok; ++j) {
           const int st = j % RING, sv = j & 1;
           if (!mbar_wait(&k_empty[st], ((j / RING) & 1) ^ 1, guard, kTimeoutProducer)) { ok = false; break; }
@@ -296,21 +298,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = uint32_t(quarter * 32) << 16;
     const int my_row = quarter * 32 + lane;
-    const bool row_ok = my_row < rows;
-    const int64_t stat_index = int64_t(head) * p.total_q + q_row + my_row;
+    const int live = rows << p.shift, fold_mask = (1 << p.shift) - 1;
+    const bool row_ok = my_row < live;
+    const int64_t stat_index = int64_t(head0 + (my_row & fold_mask)) * p.total_q + q_row + (my_row >> p.shift);
     // delta of 16 rows a warp, four elements a lane, whole rows an instruction (one row a thread took 7000
     // cycles); all loads are on their way before the first sum
     {
       const int row0 = warp * 16, e = lane * 4;
-      const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row + row0) * p.hq + head) * p.dim + e;
-      const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row + row0) * p.grad_row + head * p.grad_head + e;
+      const uint16_t* o = static_cast<const uint16_t*>(p.out) + (int64_t(q_row) * p.hq + head0) * p.dim + e;
+      const uint16_t* g = static_cast<const uint16_t*>(p.grad) + int64_t(q_row) * p.grad_row + head0 * p.grad_head + e;
       uint2 a[16], b[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         a[r] = b[r] = make_uint2(0, 0);
-        if (row0 + r < rows && e < p.dim) {
-          a[r] = *reinterpret_cast<const uint2*>(o + int64_t(r) * p.hq * p.dim);
-          b[r] = *reinterpret_cast<const uint2*>(g + r * p.grad_row);
+        const int down = row0 + r >> p.shift, across = row0 + r & fold_mask;
+        if (row0 + r < live && e < p.dim) {
+          a[r] = *reinterpret_cast<const uint2*>(o + (down * p.hq + across) * p.dim);
+          b[r] = *reinterpret_cast<const uint2*>(g + down * p.grad_row + across * p.grad_head);
         }
       }
 #pragma unroll
@@ -330,8 +334,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     const float2 nl2 = make_float2(-lse2, -lse2);
     const float2 nd2 = make_float2(-delta, -delta);
-    const int seen = row_ok ? min(span.keys, reach + my_row + 1) : 0;
-    const int seen_first = rows == ROWS ? min(span.keys, reach + 1) : 0;
+    const int seen = row_ok ? min(span.keys, reach + (my_row >> p.shift) + 1) : 0;
+    const int seen_first = rows == step ? min(span.keys, reach + 1) : 0;
     bool ok = n_tiles > 0;
     for (int j = 0; j < n_tiles && ok; ++j) {
       const int buf = j & 1;
@@ -388,18 +392,17 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       tc_fence_after_sync();
       // every product is complete: the stages lie over the Q and dO tiles
       if (half < DP / 64) {
-        const int64_t row = int64_t(q_row) + quarter * 32;
-        store_columns<FP16>(static_cast<uint16_t*>(p.dq) + (row * p.hq + head) * p.dim + half * 64, int64_t(p.hq) * p.dim,
-                            tmem_base + lane_base + C_DQ + half * 64, p.dim - half * 64, p.scale,
-                            rows - quarter * 32, n_tiles > 0, true, smem_u32(smem + warp * 4096), lane);
+        const int64_t row = int64_t(q_row) + (quarter * 32 >> p.shift);
+        store_columns<FP16>(static_cast<uint16_t*>(p.dq) + (row * p.hq + head0) * p.dim + half * 64, p.hq * p.dim, p.dim,
+                            p.shift, tmem_base + lane_base + C_DQ + half * 64, p.dim - half * 64, p.scale,
+                            live - quarter * 32, n_tiles > 0, true, smem_u32(smem + warp * 4096), lane);
       }
     }
     if (span.unit_in_sequence == -2) {  // rows behind the last sequence
-      const int words = p.dim / 8;
-      for (int i = int(threadIdx.x); i < span.rows * words; i += 256) {
-        uint16_t* dst = static_cast<uint16_t*>(p.dq) + ((int64_t(span.q0) + i / words) * p.hq + head) * p.dim + (i % words) * 8;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-      }
+      const int words = (p.dim << p.shift) / 8;
+      for (int i = int(threadIdx.x); i < span.rows * words; i += 256)
+        store16(static_cast<uint16_t*>(p.dq) + ((int64_t(span.q0) + i / words) * p.hq + head0) * p.dim + (i % words) * 8,
+                make_uint4(0, 0, 0, 0));
     }
   }
   tc_fence_before_sync();
@@ -411,10 +414,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------- dK / dV
-// With few key tiles, up to four CTAs of a cluster take a part of the group's query heads each and add
-// their accumulators at the end through each other's shared memory, in the order of their ranks: the
-// first key tile of a sequence is seen by all of its queries and would decide how long the launch takes.
-// Items are (query head of the group, block of 128 query rows that can see the tile), issued
+// With few key tiles, the two CTAs of a cluster take the items in turn and add their accumulators at
+// the end through each other's shared memory, in the order of their ranks: the first key tile of a
+// sequence is seen by all of its queries and would decide how long the launch takes.
+// Items are blocks of 128 (query row, head) pairs that can see the tile, issued
 // dV(i) | S^T(i+1) | dK(i) | dP^T(i+1): the exponentials of item i+1 run under dK(i) and dP^T(i+1), its
 // dS^T under dV(i+1) and S^T(i+2).  Single score buffers: refilling one behind the product that
 // reads its P^T / dS^T is safe, tcgen05.mma operations of one thread execute in issue order.
@@ -456,7 +459,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int member = int(blockIdx.x % unsigned(p.share));  // rank in the cluster
   const int kv_head = int((blockIdx.x / unsigned(p.share)) % unsigned(p.hkv));
   const int unit = int(blockIdx.x / (unsigned(p.share) * unsigned(p.hkv)));
-  const int my_heads = p.group / p.share, head0 = kv_head * p.group + member * my_heads;
+  const int step = ROWS >> p.shift, fold_mask = (1 << p.shift) - 1;  // query rows of an item
   const WaitGuard guard{abort_flag, p.status};
 
   if (warp == 0) {
@@ -503,10 +506,24 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int k_valid = covered ? max(0, min(ROWS, span.keys - k_first)) : 0;
   const int shift = span.keys - span.rows;                                // query i sees the keys up to i + shift
   const int i0 = max(0, k_first - shift);                                 // the first query that sees the tile
-  const int blocks = covered && k_valid > 0 && i0 < span.rows ? (span.rows - i0 + ROWS - 1) / ROWS : 0;
-  const int n_items = blocks * my_heads;
-  const int tail_rows = span.rows - i0 - (blocks - 1) * ROWS;             // queries of the last block
-  const bool ragged = blocks > 0 && tail_rows < ROWS;
+  const int blocks = covered && k_valid > 0 && i0 < span.rows ? (span.rows - i0 + step - 1) / step : 0;
+  const int all_items = blocks * (p.group >> p.shift);                    // of the cluster: heads, blocks fastest
+  const int n_items = all_items > member ? (all_items - member + p.share - 1) / p.share : 0;
+  const int tail_rows = span.rows - i0 - (blocks - 1) * step;             // queries of the last block
+  const bool ragged = blocks > 0 && tail_rows < step;
+  // block and first head of this member's first item, and how to go on to its next one
+  int block = member, head0 = kv_head * p.group;
+  auto settle = [&] {
+    while (block >= blocks) {
+      block -= blocks;
+      head0 += 1 << p.shift;
+    }
+  };
+  if (n_items > 0) settle();
+  auto advance = [&] {
+    block += p.share;
+    settle();
+  };
 
   if (warp == W_TMA) {
     if (n_items > 0) {
@@ -516,29 +533,28 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         load_tile<ATOMS>(sV, &tm_v, kv_full, kv_head, span.k0 + k_first);
       }
       bool ok = true;
-      int head = head0, block = 0;
       for (int i = 0; i < n_items && ok; ++i) {
         const int st = i % RING, sd = i & 1;
         ok = mbar_wait_w(&q_empty[st], ((i / RING) & 1) ^ 1, guard, kTimeoutProducer);
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(&q_full[st], TILE_BYTES);
-          load_tile<ATOMS>(sQ + st * TILE_BYTES, &tm_q, &q_full[st], head, span.q0 + i0 + block * ROWS);
+          load_tile<ATOMS>(sQ + st * TILE_BYTES, &tm_q, &q_full[st], head0, span.q0 + i0 + block * step);
         }
         ok = mbar_wait_w(&do_empty[sd], ((i >> 1) & 1) ^ 1, guard, kTimeoutProducer);
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(&do_full[sd], TILE_BYTES);
-          load_tile<ATOMS>(sdO + sd * TILE_BYTES, &tm_do, &do_full[sd], head, span.q0 + i0 + block * ROWS);
+          load_tile<ATOMS>(sdO + sd * TILE_BYTES, &tm_do, &do_full[sd], head0, span.q0 + i0 + block * step);
         }
         // -lse * log2(e) (or -inf: probability 0) and -delta of the item's queries
         {
           float nl[4], nd[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int q = i0 + block * ROWS + k * 32 + lane;
+            const int q = i0 + block * step + (k * 32 + lane >> p.shift);
             const bool there = q < span.rows;
-            const int64_t at = int64_t(head) * p.total_q + span.q0 + q;
+            const int64_t at = int64_t(head0 + (lane & fold_mask)) * p.total_q + span.q0 + q;
             nl[k] = there ? -p.lse[at] * LOG2E : -INFINITY;
             nd[k] = there ? -p.delta[at] : 0.f;
           }
@@ -552,20 +568,17 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           __syncwarp();
           if (lane == 0) mbar_arrive(&stats_full[sd]);
         }
-        if (++block == blocks) {
-          block = 0;
-          ++head;
-          if (ragged) {
-            ok = mbar_wait_w(&q_full[st], (i / RING) & 1, guard, kTimeoutProducer) &&
-                 mbar_wait_w(&do_full[sd], (i >> 1) & 1, guard, kTimeoutProducer);
-            if (!ok) break;
-            clear_rows<ATOMS>(smem_u32(sQ + st * TILE_BYTES), tail_rows, lane);
-            clear_rows<ATOMS>(smem_u32(sdO + sd * TILE_BYTES), tail_rows, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&clean[sd]);
-          }
+        if (ragged && block == blocks - 1) {
+          ok = mbar_wait_w(&q_full[st], (i / RING) & 1, guard, kTimeoutProducer) &&
+               mbar_wait_w(&do_full[sd], (i >> 1) & 1, guard, kTimeoutProducer);
+          if (!ok) break;
+          clear_rows<ATOMS>(smem_u32(sQ + st * TILE_BYTES), tail_rows << p.shift, lane);
+          clear_rows<ATOMS>(smem_u32(sdO + sd * TILE_BYTES), tail_rows << p.shift, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&clean[sd]);
         }
+        if (i + 1 < n_items) advance();
       }
       if (!ok || *abort_flag) {
         const uint64_t start = global_timer_ns();
@@ -577,20 +590,17 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       constexpr uint32_t idesc_s = make_idesc_16(FP16, ROWS, ROWS, 0, 0);  // 128 keys x 128 queries
       constexpr uint32_t idesc_g = make_idesc_16(FP16, ROWS, DP, 0, 1);    // 128 keys x d
       const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-      uint32_t cleaned = 0;  // bit st: parity of the stage's next cleared block
-      int block = 0;
+      uint32_t cleaned = 0;  // bit sd: parity of the stage's next cleared block
       // S^T of item i (needs its Q in shared memory; the buffer's last reader, dV(i-1), was
       // issued before).
       auto score_s = [&](int i) -> bool {
         const int st = i % RING, sd = i & 1;
         if (!mbar_wait(&q_full[st], (i / RING) & 1, guard, kTimeoutMma)) return false;
-        if (++block == blocks) {
-          block = 0;
-          if (ragged) {
-            if (!mbar_wait(&clean[sd], (cleaned >> sd) & 1, guard, kTimeoutMma)) return false;
-            cleaned ^= 1u << sd;
-          }
+        if (ragged && block == blocks - 1) {
+          if (!mbar_wait(&clean[sd], (cleaned >> sd) & 1, guard, kTimeoutMma)) return false;
+          cleaned ^= 1u << sd;
         }
+        if (i + 1 < n_items) advance();
         tc_fence_after_sync();
         const uint32_t q_addr = smem_u32(sQ + st * TILE_BYTES);
 #pragma unroll
@@ -659,16 +669,15 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int key = quarter * 32 + lane;     // key row of this thread
     bool ok = n_items > 0;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    int block = 0;
     for (int i = 0; i < n_items && ok; ++i) {
       const int st = i & 1;
-      const int q_first = i0 + block * ROWS;
-      const int q_rows = min(ROWS, span.rows - q_first);
-      if (++block == blocks) block = 0;
+      const int q_first = i0 + block * step;
+      const int q_rows = min(step, span.rows - q_first) << p.shift;  // (query row, head) pairs
+      if (i + 1 < n_items) advance();
       const uint32_t my_stats = smem_u32(stats + st * 2 * ROWS + half * 64);
       // query column c sees this key where c >= from, of the block's q_rows; only blocks that mask
       // pay for it, and the test is uniform over the CTA
-      const int from = key < k_valid ? k_first + key - shift - q_first : ROWS;
+      const int from = key < k_valid ? max(0, k_first + key - shift - q_first) << p.shift : ROWS;
       const bool plain = k_valid == ROWS && q_rows == ROWS && k_first + ROWS - 1 - shift <= q_first;
       if (!mbar_wait(&stats_full[st], (i >> 1) & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
       if (!mbar_wait(st_full, i & 1, guard, kTimeoutSoftmax)) { ok = false; break; }
@@ -744,7 +753,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
     if (ok) ok = mbar_wait(grad_done, 0, guard, kTimeoutEpilogue);
-    if ((n_items == 0 && member == 0) || (ok && p.share == 1)) {
+    if ((all_items == 0 && member == 0) || (ok && p.share == 1)) {
       tc_fence_after_sync();
       // the two halves write one gradient each; every product is complete: the stages lie over the K
       // and V tiles.  Rows that are no keys (the room behind them) get zeros.
@@ -752,7 +761,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) + (row * p.hkv + kv_head) * p.dim;
 #pragma unroll 1
       for (int c = 0; c < DP / 64; ++c)
-        store_columns<FP16>(dst + c * 64, int64_t(p.hkv) * p.dim,
+        store_columns<FP16>(dst + c * 64, p.hkv * p.dim, 0, 0,
                             tmem_base + lane_base + (half == 0 ? C_DV : C_DK) + c * 64, p.dim - c * 64,
                             half == 0 ? 1.f : p.scale, k_rows - quarter * 32, n_items > 0, key < k_valid,
                             smem_u32(smem + warp * 4096), lane);
@@ -766,7 +775,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
   }
-  if (p.share > 1 && n_items > 0) {
+  if (p.share > 1 && all_items > 0) {
     // dV and dK side by side are 2 DP columns; each member adds up `width` of them.
     const int width = 2 * DP / p.share;
     const int quarter = warp & 3, half = (warp >> 2) & 1;
@@ -785,9 +794,11 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (to == member) continue;
         const int sender = member < to ? member : member - 1;
         for (int c = half * 32; c < width; c += 64) {
-          uint32_t o[32];
-          tmem_ld_32x32(column0 + column(to * width + c), o);
-          tmem_ld_wait();
+          uint32_t o[32] = {};  // a member without items adds nothing
+          if (n_items > 0) {
+            tmem_ld_32x32(column0 + column(to * width + c), o);
+            tmem_ld_wait();
+          }
 #pragma unroll
           for (int g = 0; g < 8; ++g)
             put16_member(place(sender, key, c / 4 + g), to, make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]));
@@ -798,9 +809,11 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     if (warp < 8) {
       for (int c = half * 32; c < width; c += 64) {
         const int at = member * width + c;
-        uint32_t o[32];
-        tmem_ld_32x32(column0 + column(at), o);
-        tmem_ld_wait();
+        uint32_t o[32] = {};
+        if (n_items > 0) {
+          tmem_ld_32x32(column0 + column(at), o);
+          tmem_ld_wait();
+        }
         float sum[32];
 #pragma unroll 1
         for (int from = 0; from < p.share; ++from) {
@@ -852,7 +865,7 @@ cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap&
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(packed_dkdv_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<DP>());
   if (e != cudaSuccess) return e;
-  const int64_t q_grid = (p.total_q / ROWS + p.sequences + 1) * p.hq;
+  const int64_t q_grid = (p.total_q / (ROWS >> p.shift) + p.sequences + 1) * (p.hq >> p.shift);
   const int64_t k_units = (p.total_k / ROWS + p.sequences + 1) * p.hkv, k_grid = k_units * p.share;
   if (q_grid > 2147483647ll || k_grid > 2147483647ll) {
     set_error_detail("packed_attention: too many tiles for one launch");
@@ -879,10 +892,11 @@ cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap&
 
 cudaError_t packed_attention_bwd(const PackedArgs& a, const PackedGrads& g, cudaStream_t stream) {
   CUtensorMap tq, tdo, tk, tv;
-  if (!make_packed_map(&tq, a.q, a.dim, a.hq, a.total_q, a.q_head, a.q_row) ||
-      !make_packed_map(&tdo, g.grad, a.dim, a.hq, a.total_q, g.grad_head, g.grad_row) ||
-      !make_packed_map(&tk, a.k, a.dim, a.hkv, a.total_k, a.k_head, a.k_row) ||
-      !make_packed_map(&tv, a.v, a.dim, a.hkv, a.total_k, a.v_head, a.v_row))
+  const int shift = fold_shift(a.hq / a.hkv);
+  if (!make_packed_map(&tq, a.q, a.dim, a.hq, a.total_q, a.q_head, a.q_row, 1 << shift) ||
+      !make_packed_map(&tdo, g.grad, a.dim, a.hq, a.total_q, g.grad_head, g.grad_row, 1 << shift) ||
+      !make_packed_map(&tk, a.k, a.dim, a.hkv, a.total_k, a.k_head, a.k_row, 1) ||
+      !make_packed_map(&tv, a.v, a.dim, a.hkv, a.total_k, a.v_head, a.v_row, 1))
     return cudaErrorInvalidValue;
   BwdParams p{};
   p.q_offsets = a.q_offsets; p.k_offsets = a.k_offsets; p.k_lengths = a.k_lengths;
@@ -894,12 +908,11 @@ cudaError_t packed_attention_bwd(const PackedArgs& a, const PackedGrads& g, cuda
   p.hq = a.hq; p.hkv = a.hkv; p.group = a.hq / a.hkv; p.dim = a.dim;
   p.scale = a.scale; p.scale_log2 = a.scale * LOG2E;
   p.status = a.status;
-  // until there are two CTAs for every SM, as far as the group has heads to share out (more only add starts
-  // and ends: 198 us against 116 with four members where two give 3.5 CTAs an SM)
-  p.share = 1;
-  while (p.share < 4 && p.group % (2 * p.share) == 0 &&
-         (a.total_k / ROWS + a.sequences) * a.hkv * p.share < int64_t(2) * a.sm_count)
-    p.share *= 2;
+  p.shift = shift;
+  // Two where one CTA a key tile leaves fewer than two for every SM.  (Four were slower everywhere: 198 us
+  // against 116 for the key side of six prompts of 178 to 2045 rows, 43 against 24 for three of up to
+  // 1000: clusters of four whole SMs wait for one another to start.)
+  p.share = (a.total_k / ROWS + a.sequences) * a.hkv < int64_t(2) * a.sm_count ? 2 : 1;
   if (a.dim <= 64)
     return a.fp16 ? launch<64, true>(p, tq, tdo, tk, tv, stream) : launch<64, false>(p, tq, tdo, tk, tv, stream);
   return a.fp16 ? launch<128, true>(p, tq, tdo, tk, tv, stream) : launch<128, false>(p, tq, tdo, tk, tv, stream);

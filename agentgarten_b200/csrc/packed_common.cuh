@@ -39,27 +39,35 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// Tiles of 128 rows are (query row, head) pairs: `fold` query heads that share a key head side by side,
+// heads fastest, so that a short or ragged sequence fills them.  fold is a power of two, 1 << shift.
+__host__ __device__ __forceinline__ int fold_shift(int group) {  // of the largest power of two in the group, up to 16
+  int shift = 0;
+  while (shift < 4 && (group >> shift) % 2 == 0) ++shift;
+  return shift;
+}
+
 // 32 rows x 128 bytes of a warp from its stage in shared memory (4 KB; 16-byte word w of row r lies at word
-// w ^ (r & 7)) to global rows `pitch` bytes apart: the first `live` rows, of which `bytes` are left from
-// `dst` on.  Whole rows an instruction; stores of one row a thread would touch 32 lines each.
+// w ^ (r & 7)) to global memory: row r (of the first `live`) goes to dst + (r >> shift) * pitch + (r & (2^shift -
+// 1)) * head_pitch bytes, of which `bytes` are left from there on.  Whole rows an instruction; stores of
+// one row a thread would touch 32 lines each.
 __device__ __forceinline__ uint32_t stage_word(uint32_t stage, int row, int word) {
   return stage + row * 128 + ((word ^ row) & 7) * 16;
 }
-__device__ __forceinline__ void flush_rows(uint32_t stage, uint8_t* dst, int64_t pitch, int bytes, int live, int lane) {
+__device__ __forceinline__ void flush_rows(uint32_t stage, uint8_t* dst, int pitch, int head_pitch, int shift, int bytes,
+                                           int live, int lane) {
   __syncwarp();
   const int w = lane & 7, first = lane >> 3;
   uint4 v[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = get16(stage_word(stage, k * 4 + first, w));
   if (w * 16 < bytes) {
-    uint8_t* to = dst + first * pitch + w * 16;
-    if (live >= 32) {
+    uint8_t* to = dst + w * 16;
+    const int mask = (1 << shift) - 1;
 #pragma unroll
-      for (int k = 0; k < 8; ++k, to += 4 * pitch) store16(to, v[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k, to += 4 * pitch)
-        if (k * 4 + first < live) store16(to, v[k]);
+    for (int k = 0; k < 8; ++k) {
+      const int r = k * 4 + first;
+      if (r < live) store16(to + (r >> shift) * pitch + (r & mask) * head_pitch, v[k]);
     }
   }
   __syncwarp();

@@ -157,7 +157,7 @@ PROMPTS = [[1], [2, 1], [17], [127, 128, 129], [300, 0, 5, 514], [0], [256, 257,
 
 
 @pytest.mark.parametrize("lengths", PROMPTS)
-@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (6, 2), (8, 1)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (6, 2), (8, 1), (8, 2), (32, 1)])
 def test_attention_of_prompts(lengths, heads, kv_heads):
     _check_forward(lengths, lengths, heads, kv_heads, 128, BF16, behind=7)
 
@@ -178,7 +178,7 @@ def test_attention_of_continued_prompts(q_lengths, k_lengths, heads, kv_heads):
 
 
 @pytest.mark.parametrize("q_lengths,k_lengths", [([40, 200], [5001, 3000]), ([33], [20000]), ([100, 30, 70], [90, 8000, 1])])
-@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 1)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 1), (16, 1)])
 def test_attention_over_split_key_ranges(q_lengths, k_lengths, heads, kv_heads):
     """Few tiles against many keys: ranges of keys side by side, joined by a second launch."""
     _check_forward(q_lengths, k_lengths, heads, kv_heads, 72, BF16, room=3, behind=260)
@@ -344,7 +344,7 @@ def _check_gradients(q_lengths, k_lengths, heads, kv_heads, dim, dtype, **kw):
 
 
 @pytest.mark.parametrize("lengths", PROMPTS)
-@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (8, 1)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 3), (8, 1), (8, 2), (32, 1)])
 def test_gradients_of_prompts(lengths, heads, kv_heads):
     _check_gradients(lengths, lengths, heads, kv_heads, 128, BF16, behind=150)
 
@@ -364,7 +364,7 @@ def test_gradients_of_continued_prompts(q_lengths, k_lengths):
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 2, 64), (12, 2, 128), (6, 3, 80), (5, 5, 64)])
 @pytest.mark.parametrize("lengths", [[700], [300, 129, 40], [3000, 2900]])
 def test_gradients_with_shared_and_whole_groups(lengths, heads, kv_heads, dim):
-    """Groups whose heads are shared out over four, two or one CTA (the fewer key tiles, the more)."""
+    """Key tiles whose queries two CTAs share (few key tiles) or one CTA takes alone."""
     _check_gradients(lengths, lengths, heads, kv_heads, dim, BF16, behind=3)
 
 
