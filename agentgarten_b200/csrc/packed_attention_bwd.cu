@@ -176,6 +176,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  allow_next_launch();
   const uint32_t tmem_base = *tmem_slot;
   const PackedSpan span = *reinterpret_cast<const PackedSpan*>(span_smem);
   constexpr uint32_t C_S = 0, C_DP = 256, C_DQ = 384;
@@ -532,7 +533,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         load_tile<ATOMS>(sK, &tm_k, kv_full, kv_head, span.k0 + k_first);
         load_tile<ATOMS>(sV, &tm_v, kv_full, kv_head, span.k0 + k_first);
       }
-      bool ok = true;
+      bool ok = true, waited = false;
       for (int i = 0; i < n_items && ok; ++i) {
         const int st = i % RING, sd = i & 1;
         ok = mbar_wait_w(&q_empty[st], ((i / RING) & 1) ^ 1, guard, kTimeoutProducer);
@@ -547,7 +548,10 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           mbar_expect_tx(&do_full[sd], TILE_BYTES);
           load_tile<ATOMS>(sdO + sd * TILE_BYTES, &tm_do, &do_full[sd], head0, span.q0 + i0 + block * step);
         }
-        // -lse * log2(e) (or -inf: probability 0) and -delta of the item's queries
+        // -lse * log2(e) (or -inf: probability 0) and -delta of the item's queries; delta is the other
+        // kernel's, at whose end this one starts
+        if (!waited) after_previous_launch();
+        waited = true;
         {
           float nl[4], nd[4];
 #pragma unroll
@@ -775,6 +779,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
   }
+  after_previous_launch();
   if (p.share > 1 && all_items > 0) {
     // dV and dK side by side are 2 DP columns; each member adds up `width` of them.
     const int width = 2 * DP / p.share;
@@ -874,17 +879,19 @@ cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap&
   packed_dq_kernel<DP, FP16><<<unsigned(q_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = unsigned(p.share);
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = unsigned(p.share);
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(k_grid));
   config.blockDim = dim3(BWD_THREADS);
   config.dynamicSmemBytes = bwd_smem<DP>();
   config.stream = stream;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
   return cudaLaunchKernelEx(&config, packed_dkdv_kernel<DP, FP16>, tq, tdo, tk, tv, p);
 }
 

@@ -86,6 +86,9 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int from, int lane) {
 // A launch that may begin while the one before it still runs: its blocks take up what they can and wait
 // (after_previous_launch) before they read what that launch writes.  Every thread waits, so the
 // second launch never ends before the first.
+// `allow_next_launch`: once every block of a launch has started, the next one's may fill the SMs that
+// come free.
+__device__ __forceinline__ void allow_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void after_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
