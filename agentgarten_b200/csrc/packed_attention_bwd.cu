@@ -318,15 +318,25 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           b[r] = *reinterpret_cast<const uint2*>(g + down * p.grad_row + across * p.grad_head);
         }
       }
+      float part[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float2 x0 = unpack16<FP16>(a[r].x), x1 = unpack16<FP16>(a[r].y);
         const float2 y0 = unpack16<FP16>(b[r].x), y1 = unpack16<FP16>(b[r].y);
-        float sum = fmaf(x0.x, y0.x, fmaf(x0.y, y0.y, fmaf(x1.x, y1.x, x1.y * y1.y)));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == r) deltas[row0 + r] = sum;
+        part[r] = fmaf(x0.x, y0.x, fmaf(x0.y, y0.y, fmaf(x1.x, y1.x, x1.y * y1.y)));
       }
+      // sixteen sums over the lanes at once: every exchange halves the rows a lane still adds up
+#pragma unroll
+      for (int d = 16; d > 1; d /= 2) {
+        const bool upper = lane & d;
+#pragma unroll
+        for (int r = 0; r < d / 2; ++r) {
+          const float send = upper ? part[r] : part[r + d / 2], keep = upper ? part[r + d / 2] : part[r];
+          part[r] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+        }
+      }
+      part[0] += __shfl_xor_sync(0xffffffffu, part[0], 1);
+      if ((lane & 1) == 0) deltas[row0 + (lane >> 1)] = part[0];
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
     const float delta = deltas[my_row];
