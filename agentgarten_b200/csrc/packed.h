@@ -54,7 +54,7 @@ struct PackedArgs {
   int* status;
   // FP32 partial results of the keys' ranges: with splits > 1 the tile kernel's [splits, total_q, hq, dim]
   // and [splits, total_q, hq]; for the few-row kernel, whose ranges are chunks of `chunk` keys,
-  // [units, hkv, pieces, 16, dim] and [units, hkv, pieces, 16] with units = total_k / chunk + 3 * sequences
+  // [units, hkv, pieces, 16, dim] and [units, hkv, pieces, 16] with units = packed_rows_jobs()
   // and pieces = packed_rows_pieces(hq / hkv) (unused when total_k <= chunk).
   int splits, chunk;
   int sm_count;
@@ -62,9 +62,10 @@ struct PackedArgs {
   float* part_lse;
 };
 cudaError_t packed_attention_tiles(const PackedArgs& args, cudaStream_t stream);
-// The same function for sequences of few query rows: total_q * min(hq / hkv, 16) <= 16 * sequences.
+// The same function for few query rows; right for any.
 cudaError_t packed_attention_rows(const PackedArgs& args, cudaStream_t stream);
 int packed_rows_pieces(int group);
+int64_t packed_rows_jobs(const PackedArgs& args);  // at most, of one key head and piece
 
 // Gradient: args carries the forward's tensors (out and lse filled in); grad [total_q, hq, dim] with
 // the strides given, dq / dk / dv dense like q / k / v, delta fp32 scratch [hq, total_q].  Rows of no

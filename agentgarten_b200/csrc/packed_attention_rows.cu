@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t word_at(int row, int word) {
 
 // The sequence of a job (by_row 0: number `at`) or of a query row (by_row 1).  A sequence has `blocks`
 // blocks of 16 rows times `chunks` chunks of `length` keys: as many chunks as `p.chunk` asks for, or
-// fewer where it has several blocks, so that the jobs of all stay within total_k / chunk + 3 sequences.
+// fewer where it has several blocks, so that the jobs of all stay within packed_rows_jobs().
 // Converged warp; 32 sequences a step.  Sequences whose offsets do not fit have no jobs and no rows.
 struct JobSpan {
   int sequence;  // -1: none
@@ -407,7 +407,7 @@ cudaError_t launch(const RowsParams& p, cudaStream_t stream) {
                                              rows_smem<DP>());
   if (e != cudaSuccess) return e;
   const int64_t side = int64_t(p.hkv) * p.pieces, places = int64_t(p.sm_count) * 2;
-  const int64_t jobs = (p.total_k / p.chunk + 3 * int64_t(p.sequences)) * side;  // at most
+  const int64_t jobs = int64_t(p.most_jobs) * side;
   int64_t grid = (jobs + WARPS - 1) / WARPS;
   if (grid > places) grid = places;
   if (grid < side) grid = side;  // each of the first `side` CTAs clears rows of one head
@@ -440,11 +440,16 @@ cudaError_t packed_attention_rows(const PackedArgs& a, cudaStream_t stream) {
   p.part_out = a.part_out; p.part_lse = a.part_lse;
   p.status = a.status;
   p.sm_count = a.sm_count;
-  p.most_jobs = int(a.total_k / a.chunk + 3 * int64_t(a.sequences));
+  p.most_jobs = int(packed_rows_jobs(a));
   if (a.dim <= 64) return a.fp16 ? launch<64, true>(p, stream) : launch<64, false>(p, stream);
   return a.fp16 ? launch<128, true>(p, stream) : launch<128, false>(p, stream);
 }
 
 int packed_rows_pieces(int group) { return (group + QROWS - 1) / QROWS; }
+
+int64_t packed_rows_jobs(const PackedArgs& a) {
+  const int group = a.hq / a.hkv, heads = group < QROWS ? group : QROWS;
+  return a.total_k / a.chunk + a.total_q * heads / QROWS + 2 * int64_t(a.sequences);
+}
 
 }  // namespace agb
