@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const float* __restric
 template <int DP, bool FP16>
 cudaError_t launch_tiles(const PackedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(packed_tiles_kernel<DP, FP16>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DP>());
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_shared_memory(packed_tiles_kernel<DP, FP16>, fwd_smem<DP>(), allowed);
   if (e != cudaSuccess) return e;
   FwdParams p{};
   p.q_offsets = a.q_offsets; p.k_offsets = a.k_offsets; p.k_lengths = a.k_lengths;

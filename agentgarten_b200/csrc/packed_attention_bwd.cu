@@ -875,10 +875,9 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 template <int DP, bool FP16>
 cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap& tdo, const CUtensorMap& tk,
                    const CUtensorMap& tv, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(packed_dq_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       bwd_smem<DP>());
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(packed_dkdv_kernel<DP, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<DP>());
+  static std::atomic<uint64_t> allowed_dq{0}, allowed_dkdv{0};
+  cudaError_t e = allow_shared_memory(packed_dq_kernel<DP, FP16>, bwd_smem<DP>(), allowed_dq);
+  if (e == cudaSuccess) e = allow_shared_memory(packed_dkdv_kernel<DP, FP16>, bwd_smem<DP>(), allowed_dkdv);
   if (e != cudaSuccess) return e;
   const int64_t q_grid = (p.total_q / (ROWS >> p.shift) + p.sequences + 1) * (p.hq >> p.shift);
   const int64_t k_units = (p.total_k / ROWS + p.sequences + 1) * p.hkv, k_grid = k_units * p.share;

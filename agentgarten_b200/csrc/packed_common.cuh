@@ -11,6 +11,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace agb {
 
 // 16-byte accesses of shared memory by its own addresses (through a pointer that was aligned by hand the
@@ -81,6 +83,20 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int from, int lane) {
   for (int i = from * 8 + lane; i < 128 * 8; i += 32)
 #pragma unroll
     for (int a = 0; a < ATOMS; ++a) put16(tile + a * 16384 + i * 16, make_uint4(0, 0, 0, 0));
+}
+
+// Opts a kernel in to `bytes` of dynamic shared memory, once on every device (up to 64 of them are
+// remembered; the call itself costs the host as much as half a launch).
+template <typename Kernel>
+cudaError_t allow_shared_memory(Kernel* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // A launch that may begin while the one before it still runs: its blocks take up what they can and wait
