@@ -288,7 +288,7 @@ std::pair<Tensor, Tensor> attend(const Tensor& query, const Tensor& key, const T
   agb::PackedArgs a = packed_args(q, k, v, q_offsets, k_offsets, k_lengths, scale);
   a.out = out.data_ptr();
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
-  Tensor part_out, part_lse;
+  Tensor part_out, part_lse, part_jobs;
   const int sms = sm_count(q), group = a.hq / a.hkv;
   if (few_rows(a)) {
     const int64_t pieces = agb::packed_rows_pieces(group);
@@ -297,6 +297,8 @@ std::pair<Tensor, Tensor> attend(const Tensor& query, const Tensor& key, const T
       const int64_t slots = agb::packed_rows_jobs(a) * a.hkv * pieces * 16;
       part_out = empty_fp32({slots, a.dim}, q);
       part_lse = empty_fp32({slots}, q);
+      part_jobs = empty({a.sequences, 2}, q_offsets);
+      a.part_jobs = part_jobs.data_ptr<int>();
       a.part_out = part_out.data_ptr<float>();
       a.part_lse = part_lse.data_ptr<float>();
     }
@@ -329,11 +331,18 @@ struct PackedAttention : public torch::autograd::Function<PackedAttention> {
     const Tensor &query = saved[0], &key = saved[1], &value = saved[2], &out = saved[3], &lse = saved[4];
     const OptionalTensor k_lengths = saved[7].defined() ? OptionalTensor(saved[7]) : c10::nullopt;
     c10::cuda::CUDAGuard guard(query.device());
-    Tensor dq = empty(query.sizes(), query), dk = empty(key.sizes(), key), dv = empty(value.sizes(), value);
+    const bool key_side = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    Tensor dq = empty(query.sizes(), query), dk, dv;
+    if (key_side) {
+      dk = empty(key.sizes(), key);
+      dv = empty(value.sizes(), value);
+    }
     if (query.numel() == 0 || key.size(0) == 0 || saved[5].size(0) == 1) {
       dq.zero_();
-      dk.zero_();
-      dv.zero_();
+      if (key_side) {
+        dk.zero_();
+        dv.zero_();
+      }
     } else {
       const Tensor q = mappable(query), k = mappable(key), v = mappable(value), grad = mappable(grads[0]);
       Tensor delta = empty_fp32(lse.sizes(), lse);
@@ -345,11 +354,13 @@ struct PackedAttention : public torch::autograd::Function<PackedAttention> {
       g.grad_row = row_stride(grad);
       g.grad_head = head_stride(grad);
       g.dq = dq.data_ptr();
-      g.dk = dk.data_ptr();
-      g.dv = dv.data_ptr();
+      if (key_side) {
+        g.dk = dk.data_ptr();
+        g.dv = dv.data_ptr();
+      }
       g.delta = delta.data_ptr<float>();
       check(agb::packed_attention_bwd(a, g, stream_of(q)), "packed_attention");
-      launches += 2;
+      launches += key_side ? 2 : 1;
     }
     return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()}, "packed_attention");
   }

@@ -55,11 +55,13 @@ struct PackedArgs {
   // FP32 partial results of the keys' ranges: with splits > 1 the tile kernel's [splits, total_q, hq, dim]
   // and [splits, total_q, hq]; for the few-row kernel, whose ranges are chunks of `chunk` keys,
   // [units, hkv, pieces, 16, dim] and [units, hkv, pieces, 16] with units = packed_rows_jobs()
-  // and pieces = packed_rows_pieces(hq / hkv) (unused when total_k <= chunk).
+  // and pieces = packed_rows_pieces(hq / hkv), with the first job and the chunks of every sequence in
+  // part_jobs [sequences, 2] (unused when total_k <= chunk).
   int splits, chunk;
   int sm_count;
   float* part_out;
   float* part_lse;
+  int* part_jobs;
 };
 cudaError_t packed_attention_tiles(const PackedArgs& args, cudaStream_t stream);
 // The same function for few query rows; right for any.
@@ -73,7 +75,7 @@ int64_t packed_rows_jobs(const PackedArgs& args);  // at most, of one key head a
 struct PackedGrads {
   const void* grad;
   int64_t grad_row, grad_head;
-  void* dq; void* dk; void* dv;
+  void* dq; void* dk; void* dv;  // dk and dv may both be null: not wanted
   float* delta;
 };
 cudaError_t packed_attention_bwd(const PackedArgs& args, const PackedGrads& grads, cudaStream_t stream);

@@ -887,7 +887,7 @@ cudaError_t launch(const BwdParams& p, const CUtensorMap& tq, const CUtensorMap&
   }
   packed_dq_kernel<DP, FP16><<<unsigned(q_grid), BWD_THREADS, bwd_smem<DP>(), stream>>>(tq, tdo, tk, tv, p);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || !p.dk) return e;
   cudaLaunchAttribute attributes[2]{};
   attributes[0].id = cudaLaunchAttributeClusterDimension;
   attributes[0].val.clusterDim.x = unsigned(p.share);

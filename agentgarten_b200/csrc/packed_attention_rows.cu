@@ -43,6 +43,7 @@ struct RowsParams {
   int hq, hkv, group, dim, pieces, chunk;
   float scale_log2;
   float* part_out; float* part_lse;
+  int* part_jobs;
   int sm_count, most_jobs;
   int* status;
 };
@@ -78,20 +79,20 @@ __device__ __forceinline__ uint32_t word_at(int row, int word) {
   return uint32_t(row * DP * 2 + ((word & ~7) | ((word ^ row) & 7)) * 16);
 }
 
-// The sequence of a job (by_row 0: number `at`) or of a query row (by_row 1).  A sequence has `blocks`
+// The sequence of job number `at`.  A sequence has `blocks`
 // blocks of 16 rows times `chunks` chunks of `length` keys: as many chunks as `p.chunk` asks for, or
 // fewer where it has several blocks, so that the jobs of all stay within packed_rows_jobs().
-// Converged warp; 32 sequences a step.  Sequences whose offsets do not fit have no jobs and no rows.
+// Converged warp; 32 sequences a step.  Sequences whose offsets do not fit have no jobs.  A warp's job
+// numbers rise: the search goes on from where the last one ended (`base`, with `before` jobs behind it).
 struct JobSpan {
   int sequence;  // -1: none
   int first, chunks, length;
   int q0, rows, k0, keys;
 };
-__device__ inline JobSpan find_job(int at, bool by_row, int heads, const RowsParams& p, int* status) {
+__device__ inline JobSpan find_job(int at, int heads, int& base, int& before, const RowsParams& p, int* status) {
   const int lane = threadIdx.x & 31;
   JobSpan span{-1, 0, 0, 0, 0, 0, 0, 0};
-  int before = 0;  // jobs of earlier sequences
-  for (int base = 0; base < p.sequences; base += 32) {
+  for (; base < p.sequences; base += 32) {
     const int s = base + lane;
     const bool there = s < p.sequences;
     const int q0 = p.q_offsets[there ? s : 0], q1 = p.q_offsets[there ? s + 1 : 0];
@@ -113,7 +114,7 @@ __device__ inline JobSpan find_job(int at, bool by_row, int heads, const RowsPar
       const int other = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += other;
     }
-    const bool here = jobs > 0 && (by_row ? at >= q0 && at < q1 : at < before + sum);
+    const bool here = jobs > 0 && at < before + sum;
     const unsigned votes = __ballot_sync(0xffffffffu, here);
     if (votes) {
       const int owner = __ffs(votes) - 1;
@@ -149,14 +150,19 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
     }
   }
   // neighbouring warps take the same keys of neighbouring heads
+  int base = 0, before = 0;
   for (int64_t job = int64_t(blockIdx.x) * WARPS + warp;; job += int64_t(gridDim.x) * WARPS) {
   const int unit = divide(int(job), side), rest = int(job) - unit * side;
   const int kv_head = divide(rest, p.pieces), piece = rest - kv_head * p.pieces;
   const int head0 = kv_head * p.group + piece * QROWS;
   const int heads = min(QROWS, p.group - piece * QROWS);  // query heads side by side in the rows
   // the pieces of a group have the same jobs: those of its first
-  const JobSpan span = find_job(unit, false, min(QROWS, p.group), p, p.status);
+  const JobSpan span = find_job(unit, min(QROWS, p.group), base, before, p, p.status);
   if (span.sequence < 0) return;
+  if (unit == span.first && rest == 0 && lane == 0 && p.part_jobs) {  // for the join
+    p.part_jobs[2 * span.sequence] = span.first;
+    p.part_jobs[2 * span.sequence + 1] = span.chunks;
+  }
   if (unit >= p.most_jobs) {  // offsets that fall make sequences overlap: more jobs than partial results
     if (lane == 0 && p.status) atomicCAS(p.status, 0, kBadIndex);
     return;
@@ -332,17 +338,32 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) packed_rows_join_kernel(const
   __shared__ float weight[JOIN_WARPS], tops[JOIN_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int row = int(blockIdx.x / unsigned(p.hq)), head = int(blockIdx.x % unsigned(p.hq));
-  const JobSpan span = find_job(row, true, min(QROWS, p.group), p, nullptr);
+  // the sequence of the row: 32-way search for the last s with q_offsets[s] <= row
+  int low = 0;
+  for (int count = p.sequences; count > 0;) {
+    const int stride = (count + 31) / 32;
+    const bool reached = lane * stride < count && p.q_offsets[low + lane * stride] <= row;
+    const unsigned votes = __ballot_sync(0xffffffffu, reached);
+    if (votes == 0) break;
+    const int last = 31 - __clz(votes), behind = count - last * stride;
+    low += last * stride;
+    count = stride == 1 ? 0 : (behind < stride ? behind : stride);
+  }
+  const int q0 = p.q_offsets[low], q1 = p.q_offsets[low + 1], k0 = p.k_offsets[low], k1 = p.k_offsets[low + 1];
+  const int keys = p.k_lengths ? p.k_lengths[low] : k1 - k0;
+  const bool fits = q0 >= 0 && row >= q0 && row < q1 && q1 <= p.total_q && k0 >= 0 && k1 >= k0 && k1 <= p.total_k &&
+                    keys >= 0 && keys <= k1 - k0;
   const int kv_head = head / p.group, in_group = head % p.group;
   const int piece = in_group / QROWS;
   const int heads = min(QROWS, p.group - piece * QROWS);
-  const int chunks = span.chunks;
   after_previous_launch();
-  // written by the first launch, or never (offsets that do not fit)
-  if (span.sequence < 0 || chunks <= 1 || span.first + chunks * ((span.rows * heads + QROWS - 1) / QROWS) > p.most_jobs) return;
-  const int f = (row - span.q0) * heads + in_group % QROWS;
+  if (!fits) return;
+  const int first_job = p.part_jobs[2 * low], chunks = p.part_jobs[2 * low + 1];
+  // written by the first launch, or never (offsets that fall)
+  if (chunks <= 1 || first_job + chunks * (((q1 - q0) * heads + QROWS - 1) / QROWS) > p.most_jobs) return;
+  const int f = (row - q0) * heads + in_group % QROWS;
   const int64_t step = int64_t(p.hkv) * p.pieces * QROWS;
-  const int64_t first = ((int64_t(span.first) + f / QROWS * chunks) * p.hkv * p.pieces + kv_head * p.pieces + piece) * QROWS +
+  const int64_t first = ((int64_t(first_job) + f / QROWS * chunks) * p.hkv * p.pieces + kv_head * p.pieces + piece) * QROWS +
                         f % QROWS;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.f, high = -INFINITY;
@@ -437,7 +458,7 @@ cudaError_t packed_attention_rows(const PackedArgs& a, cudaStream_t stream) {
   p.pieces = packed_rows_pieces(p.group);
   p.chunk = a.chunk;
   p.scale_log2 = a.scale * LOG2E;
-  p.part_out = a.part_out; p.part_lse = a.part_lse;
+  p.part_out = a.part_out; p.part_lse = a.part_lse; p.part_jobs = a.part_jobs;
   p.status = a.status;
   p.sm_count = a.sm_count;
   p.most_jobs = int(packed_rows_jobs(a));

@@ -154,9 +154,10 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     : k_offsets[s + 1]`` (default: its query rows).  Its queries are the *last* rows of its keys:
     query ``i`` of ``n`` sees the keys up to ``keys - n + i``.  A query that sees no key gives zeros,
     and so do rows behind the last sequence.  What lies in key rows that belong to no sequence, to
-    another one or behind ``k_lengths`` has no influence, whatever it holds; a NaN or an infinity
-    among a sequence's own keys may spread to earlier queries of the sequence in the same tile of
-    128 rows.
+    another one or behind ``k_lengths`` has no influence, whatever it holds.  A NaN or an infinity
+    among a sequence's own rows may spread within that sequence: a value to queries that stop short
+    of it within the same 128 keys, and in the gradient a query to keys behind it within the same
+    tile of queries.
 
     The offsets stay on the device.  The kernels check them; a sequence whose offsets do not fit is
     skipped and reported through the kernel status word.  ``scale`` defaults to ``dim ** -0.5``.
