@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) packed_rows_kernel(const RowsPa
       *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = make_uint4(0, 0, 0, 0);
     }
   }
+  allow_next_launch();  // the join's blocks take the places of the first to end
   // neighbouring warps take the same keys of neighbouring heads
   int base = 0, before = 0;
   for (int64_t job = int64_t(blockIdx.x) * WARPS + warp;; job += int64_t(gridDim.x) * WARPS) {
