@@ -240,11 +240,22 @@ bool few_rows(const agb::PackedArgs& a) {
   return a.total_q * std::min(a.hq / a.hkv, 16) <= int64_t(32) * a.sequences;
 }
 
-// Keys of a chunk: about three for every warp that the GPU holds (eight an SM), and not so few that
-// starting and joining them shows.
+// Keys of a chunk.  Eight warps an SM take one job each at a time.  Where chunks of at most 512 keys give no
+// more jobs than that, just such chunks: a job is a chain of loads, and there is no second one to hide
+// its end.  Longer ones would leave uneven caches with a long tail, so there about three jobs for every
+// warp.  Per call, this rule against three jobs of at least 128 keys, 32 query and 8 key heads of 128: one
+// token against 500 / 4000 / 32000 / 38000 keys 11.3 : 14.8, 13.8 : 15.4, 35.1 : 37.4, 37.9 : 45.1 us; 16 tokens
+// against 1200 each 23 : 28, 32 against 1000 each 34.2 : 35.8; eight prompts of 8 rows on 1000, the one that
+// lost, 25.6 : 25.1.
 int rows_chunk(const agb::PackedArgs& a, int sms) {
-  const int64_t work = a.total_k * a.hkv * agb::packed_rows_pieces(a.hq / a.hkv);
-  const int64_t chunk = (work / (int64_t(sms) * 8 * 3) + 63) / 64 * 64;
+  const int64_t side = int64_t(a.hkv) * agb::packed_rows_pieces(a.hq / a.hkv), warps = int64_t(sms) * 8;
+  if (a.total_k <= int64_t(128) * a.sequences) return 128;
+  const int64_t spare = warps - a.sequences * side;  // a sequence's last chunk is a short one
+  if (2 * spare >= warps) {
+    const int64_t once = (a.total_k * side + spare - 1) / spare;
+    if (once <= 512) return int((std::max<int64_t>(once, 32) + 31) / 32 * 32);
+  }
+  const int64_t chunk = (a.total_k * side / (3 * warps) + 63) / 64 * 64;
   return int(std::min<int64_t>(std::max<int64_t>(chunk, 128), 8192));
 }
 
