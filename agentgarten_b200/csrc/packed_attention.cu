@@ -27,7 +27,7 @@
 // What bounds it: 2048 cycles of products for a pair of 128 x 128 tiles against about 1600 of one
 // tile's softmax, which has to lie between two of its products (2900 cycles measured).  With 32 query and 8
 // key heads of 128: 435 us for a prompt of 8192 (1.26 PFLOP/s, tensor pipe active 63 % of the cycles), 1654 us
-// for one of 16384 (1.33 PFLOP/s; 1930 in calls without a pause, at the clocks that the power limit leaves).
+// for one of 16384 (1.33 PFLOP/s; 1880 to 1930 in calls without a pause, at the clocks that the power limit leaves).
 //
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512); P_t over the first half of S_t.
 #include "agb.h"

@@ -11,9 +11,10 @@
 //                S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
 // Shared heads are summed in the accumulators, in FP32.  P and dS are rounded to the tensors' type
 // on their way into the tensor core (scale stays out of dS and is applied to the sums, which keeps
-// small dS of fp16 above its underflow).  Rows of a tile that belong to no one or to another
-// sequence are cleared in shared memory before a product sums over them, so what they hold never
-// spreads.
+// small dS of fp16 above its underflow).  That rounding of dS takes the relative error of dq and dk in
+// bf16 from the result's own 0.0017 to 0.0023; delta comes from the rounded O, which makes it 0.0027
+// (200 rows).  Rows of a tile that belong to no one or to another sequence are cleared in shared memory
+// before a product sums over them, so what they hold never spreads.
 //
 // Why two kernels of whole 128 x 128 blocks: dQ sums over keys and dK, dV over queries, and one kernel for
 // both would add one of them up in memory with atomics.  The price is S and dP computed twice, seven

@@ -14,8 +14,8 @@
 // the GPU holds: a cache has room that nobody uses yet, and a block for every chunk of that room
 // cost as much as half of the real ones.
 //
-// With 32 query and 8 key heads of 128: one token against 131071 keys (537 MB) 87 us, 6.1 TB/s, and 99 with
-// the join; 24 tokens against caches of 60 to 8191 keys (184 MB) 38 us, 4.8 TB/s, and 46 with the join.
+// With 32 query and 8 key heads of 128: one token against 131071 keys (537 MB) 87 us, 6.1 TB/s, and 97 with
+// the join; 24 tokens against caches of 60 to 8191 keys (184 MB) 38 us, 4.8 TB/s, and 45 with the join.
 #include "agb.h"
 #include "packed.h"
 #include "packed_common.cuh"
